@@ -19,6 +19,8 @@
  * written; the output is fully overwritten and nothing outside it is touched; work is
  * issued asynchronously on the legacy default stream of the current device and the
  * functions return void - poll cudaGetLastError() and synchronise before reading results.
+ * (The dynamic-quantisation operators at the end of this file take the stream as an argument,
+ * return a code and use no scratch memory.)
  * Scratch memory is owned by the library (per device, grow-only, never freed).  Calls are
  * not thread-safe.
  */
@@ -287,6 +289,68 @@ double texo_f16_issue_rate_tflops(int pairs, int batches, int per_commit);
  * boxes, bit 1 = B boxes.  Synchronises. */
 double texo_int8_feed_rate_tbs(const void* A, const void* B, int M, int N, int K, int stages,
                                int mode);
+
+/* ---- dynamic quantisation: one activation scale per token -----------------------------
+ *
+ * The producers write int8 activations and their scales, the product takes them and gives
+ * floating values back.  None of these has a counterpart in the reference, whose quantised
+ * operators take one activation scale per tensor (src/mm_int8.cu:530-535).
+ *
+ * `stream` is a cudaStream_t; null is the legacy default stream.  The work is issued on it
+ * asynchronously; there is no scratch memory, so calls on different streams may overlap, and
+ * calls may be captured into a graph (after one call per device outside of capture, which
+ * sets the device up; a capturing call before that returns -4).  Returns 0, -1 bad arguments, -3 a launch was refused,
+ * -4 first call of this device while capturing.  Element types: */
+#define TEXO_F16 0
+#define TEXO_BF16 1
+#define TEXO_F32 2
+
+/* Y[m,n] = round(float(sum_k A[m,k] B[k,n]) * scale_A[m] * scale_B[n] + bias[n]).
+ * A [M,K], B [K,N] int8; scale_A [M], scale_B [N], bias [N] (or null: no addition) FP32; Y [M,N]
+ * of type out_type.  The dot is exact for every K; then FP32: one rounding of the dot, one of
+ * dot * scale_A, one of the product with scale_B plus bias (fused), one to Y's type.  M, N > 0,
+ * K >= 0 (K == 0: A and B may be null).  Any byte alignment of A and B; Y, the scales and the
+ * bias are aligned to their elements.  Y overlaps no input. */
+int texo_mm_int8_solve_per_token(const int8_t* A, const int8_t* B, void* Y, int M, int N, int K,
+                                 const float* scale_A, const float* scale_B, const float* bias,
+                                 int out_type, void* stream);
+/* Path of the last call: 1 = SIMT kernel (K = 0, K >= 2^17, other GPUs). */
+int texo_mm_int8_per_token_last_path(void);
+void texo_mm_int8_per_token_force_path(int path);
+
+/* The norms before and after a transformer block, fused with the block's gate and the residual
+ * add:
+ *   u = x, or x * rsqrt(mean_j(x^2) + eps) * post_weight   (post_weight may be null)
+ *   u = u * gate                                           (gate may be null)
+ *   z = residual_scale * residual + u
+ *   y = z * rsqrt(mean_j(z^2) + eps) * weight
+ * x, y [N,C] of type x_type; residual, z [N,C] of residual_type (x_type or TEXO_F32); weight,
+ * post_weight [C] and gate FP32 if weights_f32, else x_type.  gate: gate_rows rows, each for
+ * N / gate_rows consecutive tokens (gate_rows divides N), of C values if gate_per_channel, else
+ * of one.  FP32 throughout; z is rounded to its type in memory, y comes from the unrounded z.  z
+ * may be residual and y may be x (same address); otherwise outputs overlap no input. */
+int texo_block_norm_solve(const void* x, const void* residual, const void* weight,
+                          const void* post_weight, const void* gate, void* y, void* z, int N, int C,
+                          int gate_rows, int gate_per_channel, float eps, float residual_scale,
+                          int x_type, int residual_type, int weights_f32, void* stream);
+/* The same with y quantised per token: scale [N] FP32, q [N,C] int8,
+ *   scale = max(max_j |y|, 2^-100) / 127,   q = rint(y * (127 / max(max_j |y|, 2^-100)))
+ * (within [-127, 127]).  A row whose y holds a NaN or an infinity gets scale NaN and q = 0. */
+int texo_block_norm_quant_solve(const void* x, const void* residual, const void* weight,
+                                const void* post_weight, const void* gate, int8_t* q, float* scale,
+                                void* z, int N, int C, int gate_rows, int gate_per_channel, float eps,
+                                float residual_scale, int x_type, int residual_type, int weights_f32,
+                                void* stream);
+
+/* The per-token quantiser alone: y = x [N,C] of type x_type, rows row_stride elements apart. */
+int texo_quant_per_token_solve(const void* x, int8_t* q, float* scale, int N, int C,
+                               long long row_stride, int x_type, void* stream);
+/* The same behind the SwiGLU product: y[n,j] = silu(gate[n,j]) * up[n,j], q [N,F].  gate_up has
+ * 2F values per row: gate j and up j at 2j and 2j+1 if interleaved (the column order of
+ * texo_mm_int8_swiglu_solve), else at j and F+j. */
+int texo_swiglu_quant_per_token_solve(const void* gate_up, int8_t* q, float* scale, int N, int F,
+                                      long long row_stride, int interleaved, int x_type,
+                                      void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,6 +1,6 @@
 """B200-native quantized matmul operators behind the reference's `solve` C ABI.
 
-  texo_b200.ops       mm_int8 / mm_int4 / dequantization on torch CUDA tensors
+  texo_b200.ops       the operators on torch CUDA tensors
   texo_b200.sharded   column-sharded multi-GPU forms (one process per GPU)
   texo_b200.build     in-tree nvcc build of the libraries (sm_100a)
 """

@@ -13,7 +13,9 @@ from . import _lib
 
 __all__ = ["mm_int8", "mm_int8_per_channel", "mm_int8_per_group", "mm_int8_swiglu", "mm_int8_dequant", "mm_int4",
            "mm_int4a8", "mm_int4a8_per_channel", "mm_int4a8_per_group", "dequantization", "rms_norm_w_residual",
-           "rms_norm_quant", "mm_int8_host", "Int8Weights", "last_path", "status", "force_path"]
+           "rms_norm_quant", "mm_int8_host", "Int8Weights", "mm_int8_per_token", "block_norm",
+           "block_norm_quant_per_token", "quant_per_token", "swiglu_quant_per_token", "last_path", "status",
+           "force_path"]
 
 
 def _check_cuda(name: str, t: torch.Tensor, dtype: torch.dtype) -> None:
@@ -446,6 +448,200 @@ class Int8Weights:
             self.close()
         except Exception:
             pass
+
+
+# ---- dynamic quantisation: one activation scale per token.  These run on the caller's current
+# torch stream (the C entry points take it as an argument), use no scratch memory and may be
+# captured into a CUDA graph once the same call has been made outside of capture.
+
+_TYPE_CODES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+def _check_float(name: str, t: torch.Tensor) -> int:
+    """Checks a contiguous floating CUDA tensor and returns the library's code of its type."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (there is no CPU path)")
+    code = _TYPE_CODES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{name} must be float16, bfloat16 or float32, got {t.dtype}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous and row-major")
+    return code
+
+
+def _check_out(name: str, t: torch.Tensor | None, shape: tuple, dtype: torch.dtype,
+               like: torch.Tensor) -> torch.Tensor:
+    """The output tensor: a new one, or the caller's after its checks."""
+    if t is None:
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    _check_cuda(name, t, dtype)
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} has the wrong shape")
+    return t
+
+
+def _call_on_stream(name: str, like: torch.Tensor, others: tuple, *args) -> None:
+    """Calls a stream-taking entry point on `like`'s device and that device's current stream."""
+    device = like.device
+    for t in others:
+        if t is not None and t.device != device:
+            raise ValueError("all tensors must be on the same device")
+    fn = getattr(_lib.load(), name)
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, stream)
+    if rc == -4:
+        raise RuntimeError(f"{name}: make one call on this device before capturing a graph")
+    if rc != 0:
+        raise RuntimeError(f"{name} failed with code {rc}")
+
+
+def _ptr(t: torch.Tensor | None):
+    return None if t is None else t.data_ptr()
+
+
+def mm_int8_per_token(A: torch.Tensor, B: torch.Tensor, scale_A: torch.Tensor, scale_B: torch.Tensor,
+                      bias: torch.Tensor | None = None, out_dtype: torch.dtype = torch.float16,
+                      out: torch.Tensor | None = None) -> torch.Tensor:
+    """Y[M,N] = float(sum_k A[m,k] B[k,n]) * scale_A[m] * scale_B[n] (+ bias[n]), rounded once to
+    out_dtype (float16, bfloat16 or float32).  A [M,K], B [K,N] int8; scale_A [M], scale_B [N],
+    bias [N] float32, as quant_per_token and its relatives write them.  The dot is exact."""
+    _check_cuda("A", A, torch.int8)
+    _check_cuda("B", B, torch.int8)
+    _check_cuda("scale_A", scale_A, torch.float32)
+    _check_cuda("scale_B", scale_B, torch.float32)
+    if A.dim() != 2 or B.dim() != 2 or A.shape[1] != B.shape[0]:
+        raise ValueError(f"shape mismatch: A {tuple(A.shape)} B {tuple(B.shape)}")
+    M, K = A.shape
+    N = B.shape[1]
+    if N <= 0 or scale_A.shape != (M,) or scale_B.shape != (N,):
+        raise ValueError("N must be positive, scale_A must be [M] and scale_B [N]")
+    if bias is not None:
+        _check_cuda("bias", bias, torch.float32)
+        if bias.shape != (N,):
+            raise ValueError("bias must be [N]")
+    code = _TYPE_CODES.get(out_dtype)
+    if code is None:
+        raise ValueError(f"out_dtype must be float16, bfloat16 or float32, got {out_dtype}")
+    out = _check_out("out", out, (M, N), out_dtype, A)
+    if M > 0:
+        _call_on_stream("texo_mm_int8_solve_per_token", A, (B, scale_A, scale_B, bias, out),
+                        A.data_ptr() if K else None, B.data_ptr() if K else None, out.data_ptr(), M, N, K,
+                        scale_A.data_ptr(), scale_B.data_ptr(), _ptr(bias), code)
+    return out
+
+
+def _block_norm(quant, x, residual, weight, eps, post_weight, gate, residual_scale, out, scale_out, z_out):
+    x_code = _check_float("x", x)
+    residual_code = _check_float("residual", residual)
+    weight_code = _check_float("weight", weight)
+    if x.dim() != 2 or residual.shape != x.shape or x.shape[1] <= 0 or weight.shape != (x.shape[1],):
+        raise ValueError("x, residual must be [N, C] with C > 0 and weight [C]")
+    N, C = x.shape
+    if residual_code not in (x_code, 2):
+        raise ValueError("residual must have x's type or float32")
+    if weight_code not in (x_code, 2):
+        raise ValueError("weight must have x's type or float32")
+    if post_weight is not None:
+        _check_cuda("post_weight", post_weight, weight.dtype)
+        if post_weight.shape != (C,):
+            raise ValueError("post_weight must be [C]")
+    gate_rows, gate_per_channel = 1, 1
+    if gate is not None:
+        _check_cuda("gate", gate, weight.dtype)
+        if gate.dim() == 1:
+            ok, gate_rows = gate.shape == (C,), 1
+        else:
+            gate_rows = gate.shape[0]
+            ok = gate.dim() == 2 and gate.shape[1] in (1, C) and (N == 0 or (gate_rows > 0 and N % gate_rows == 0))
+            gate_per_channel = int(ok and gate.shape[1] == C)
+        if not ok:
+            raise ValueError("gate must be [C], [R, C] or [R, 1] with R dividing N")
+    out = _check_out("out", out, (N, C), torch.int8 if quant else x.dtype, x)
+    z = _check_out("z_out", z_out, (N, C), residual.dtype, x)
+    scale = _check_out("scale_out", scale_out, (N,), torch.float32, x) if quant else None
+    if N > 0:
+        name = "texo_block_norm_quant_solve" if quant else "texo_block_norm_solve"
+        outs = (out.data_ptr(), scale.data_ptr()) if quant else (out.data_ptr(),)
+        _call_on_stream(name, x, (residual, weight, post_weight, gate, out, z, scale), x.data_ptr(),
+                        residual.data_ptr(), weight.data_ptr(), _ptr(post_weight), _ptr(gate), *outs, z.data_ptr(),
+                        N, C, gate_rows, gate_per_channel, eps, residual_scale, x_code, residual_code,
+                        int(weight_code == 2))
+    return (out, scale, z) if quant else (out, z)
+
+
+def block_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float,
+               post_weight: torch.Tensor | None = None, gate: torch.Tensor | None = None,
+               residual_scale: float = 1.0, out: torch.Tensor | None = None,
+               z_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The norms around a transformer block in one pass.  x [N,C] is the block's output, residual
+    [N,C] the stream it is added to:
+      u = x, or its RMSNorm times post_weight;  u = u * gate;  z = residual_scale * residual + u;
+      y = RMSNorm(z) * weight.  Returns (y, z).
+    x float16, bfloat16 or float32; residual x's type or float32; weight x's type or float32, and
+    post_weight [C] and gate ([C], [R,C] or [R,1], a row for N / R consecutive tokens) of its
+    type.  y has x's type, z residual's; FP32 in between.  z_out may be residual, out may be x."""
+    return _block_norm(False, x, residual, weight, eps, post_weight, gate, residual_scale, out, None, z_out)
+
+
+def block_norm_quant_per_token(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float,
+                               post_weight: torch.Tensor | None = None, gate: torch.Tensor | None = None,
+                               residual_scale: float = 1.0, out: torch.Tensor | None = None,
+                               scale_out: torch.Tensor | None = None, z_out: torch.Tensor | None = None
+                               ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """block_norm with y quantised for mm_int8_per_token: returns (q int8 [N,C], scale float32
+    [N], z), y ~ q * scale with scale = max(max|y|, 2^-100) / 127 per token.  A row that holds a
+    NaN or an infinity gets scale NaN and q = 0."""
+    return _block_norm(True, x, residual, weight, eps, post_weight, gate, residual_scale, out, scale_out, z_out)
+
+
+def _check_rows(name: str, t: torch.Tensor) -> int:
+    """Like _check_float, but rows may be any distance apart (a slice of a wider matrix)."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (there is no CPU path)")
+    code = _TYPE_CODES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{name} must be float16, bfloat16 or float32, got {t.dtype}")
+    if t.dim() != 2 or t.shape[1] <= 0:
+        raise ValueError(f"{name} must be a matrix with at least one column")
+    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        raise ValueError(f"{name} must be row-major with rows that do not overlap")
+    return code
+
+
+def quant_per_token(x: torch.Tensor, out: torch.Tensor | None = None,
+                    scale_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """(q int8 [N,C], scale float32 [N]) with x ~ q * scale: scale = max(max|x|, 2^-100) / 127 per
+    row, q = rint(x / scale).  x float16, bfloat16 or float32, rows any distance apart.  A row
+    that holds a NaN or an infinity gets scale NaN and q = 0."""
+    code = _check_rows("x", x)
+    N, C = x.shape
+    q = _check_out("out", out, (N, C), torch.int8, x)
+    scale = _check_out("scale_out", scale_out, (N,), torch.float32, x)
+    if N > 0:
+        _call_on_stream("texo_quant_per_token_solve", x, (q, scale), x.data_ptr(), q.data_ptr(), scale.data_ptr(),
+                        N, C, max(x.stride(0), C), code)
+    return q, scale
+
+
+def swiglu_quant_per_token(gate_up: torch.Tensor, interleaved: bool = True, out: torch.Tensor | None = None,
+                           scale_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """quant_per_token(silu(gate) * up) for gate_up [N, 2F]: gate and up columns interleaved (gate
+    j at 2j, up j at 2j + 1, the order of mm_int8_swiglu's weights) or side by side.  Returns (q
+    int8 [N,F], scale float32 [N])."""
+    code = _check_rows("gate_up", gate_up)
+    N, F = gate_up.shape[0], gate_up.shape[1] // 2
+    if gate_up.shape[1] % 2:
+        raise ValueError("gate_up must have an even number of columns")
+    q = _check_out("out", out, (N, F), torch.int8, gate_up)
+    scale = _check_out("scale_out", scale_out, (N,), torch.float32, gate_up)
+    if N > 0:
+        _call_on_stream("texo_swiglu_quant_per_token_solve", gate_up, (q, scale), gate_up.data_ptr(), q.data_ptr(),
+                        scale.data_ptr(), N, F, max(gate_up.stride(0), 2 * F), int(bool(interleaved)), code)
+    return q, scale
 
 
 def last_path(op: str = "mm_int8") -> int:
