@@ -314,7 +314,10 @@ double texo_int8_feed_rate_tbs(const void* A, const void* B, int M, int N, int K
 int texo_mm_int8_solve_per_token(const int8_t* A, const int8_t* B, void* Y, int M, int N, int K,
                                  const float* scale_A, const float* scale_B, const float* bias,
                                  int out_type, void* stream);
-/* Path of the last call: 1 = SIMT kernel (K = 0, K >= 2^17, other GPUs). */
+/* Path of the last call: 1 = SIMT kernel (K = 0, K >= 2^17, other GPUs), 2 = streaming tcgen05
+ * kernel (few rows or few tiles), 3 = the same with operands that TMA cannot move (K or N not a
+ * multiple of 16, A or B not 16-byte aligned), 4 = CTA-pair tcgen05 kernel.  force_path (0 =
+ * automatic) is for diagnostics; a path whose preconditions do not hold is not taken. */
 int texo_mm_int8_per_token_last_path(void);
 void texo_mm_int8_per_token_force_path(int path);
 

@@ -46,12 +46,18 @@ inline void note_host_error(int code) {
   if (host_status() == 0) host_status() = code;
 }
 
-inline DeviceCtx& device_ctx() {
+// The current device's entry, set up or not.
+inline DeviceCtx& device_ctx_entry(int& device) {
   static DeviceCtx table[MAX_DEVICES];
-  int device = 0;
+  device = 0;
   cudaGetDevice(&device);
   if (device < 0 || device >= MAX_DEVICES) device = 0;
-  DeviceCtx& ctx = table[device];
+  return table[device];
+}
+
+inline DeviceCtx& device_ctx() {
+  int device;
+  DeviceCtx& ctx = device_ctx_entry(device);
   if (!ctx.ready) {
     ctx.device = device;
     cudaDeviceGetAttribute(&ctx.sm_count, cudaDevAttrMultiProcessorCount, device);
@@ -61,6 +67,13 @@ inline DeviceCtx& device_ctx() {
     ctx.ready = true;
   }
   return ctx;
+}
+
+// Whether `stream` is being captured into a graph, where set-up that allocates must not run.
+inline bool is_capturing(cudaStream_t stream) {
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(stream, &capture) != cudaSuccess) cudaGetLastError();
+  return capture != cudaStreamCaptureStatusNone;
 }
 
 // Grow-only scratch (first call / growth allocates; steady state does not).
