@@ -20,7 +20,7 @@
  * issued asynchronously on the legacy default stream of the current device and the
  * functions return void - poll cudaGetLastError() and synchronise before reading results.
  * (The dynamic-quantisation operators at the end of this file take the stream as an argument,
- * return a code and use no scratch memory.)
+ * return a code and own no scratch memory.)
  * Scratch memory is owned by the library (per device, grow-only, never freed).  Calls are
  * not thread-safe.
  */
@@ -297,7 +297,7 @@ double texo_int8_feed_rate_tbs(const void* A, const void* B, int M, int N, int K
  * operators take one activation scale per tensor (src/mm_int8.cu:530-535).
  *
  * `stream` is a cudaStream_t; null is the legacy default stream.  The work is issued on it
- * asynchronously; there is no scratch memory, so calls on different streams may overlap, and
+ * asynchronously; the library owns no scratch memory for it, so calls on different streams may overlap, and
  * calls may be captured into a graph (after one call per device outside of capture, which
  * sets the device up; a capturing call before that returns -4).  Returns 0, -1 bad arguments, -3 a launch was refused,
  * -4 first call of this device while capturing.  Element types: */
@@ -313,7 +313,14 @@ double texo_int8_feed_rate_tbs(const void* A, const void* B, int M, int N, int K
  * bias are aligned to their elements.  Y overlaps no input. */
 int texo_mm_int8_solve_per_token(const int8_t* A, const int8_t* B, void* Y, int M, int N, int K,
                                  const float* scale_A, const float* scale_B, const float* bias,
-                                 int out_type, void* stream);
+                                 int out_type, void* workspace, long long workspace_bytes,
+                                 void* stream);
+/* Bytes of workspace (device memory, 16-byte aligned) with which the call would make copies of
+ * operands that TMA cannot move (K or N not a multiple of 16, A or B not 16-byte aligned), rows
+ * padded, because that is faster than gathering them; 0 if it would not.  The workspace is
+ * optional: without it, or with less of it, the call gathers.  It is free again once the call's
+ * work has run.  0 too before the device's first call. */
+long long texo_mm_int8_per_token_workspace(const int8_t* A, const int8_t* B, int M, int N, int K);
 /* Path of the last call: 1 = SIMT kernel (K = 0, K >= 2^17, other GPUs), 2 = streaming tcgen05
  * kernel (few rows or few tiles), 3 = the same with operands that TMA cannot move (K or N not a
  * multiple of 16, A or B not 16-byte aligned), 4 = CTA-pair tcgen05 kernel.  force_path (0 =

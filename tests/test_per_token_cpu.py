@@ -17,7 +17,7 @@ PTR = ctypes.c_void_p(4096)  # never dereferenced: every call here is refused
 
 
 def test_mm_entry_point_refuses(lib):
-    good = [PTR, PTR, PTR, 4, 32, 16, PTR, PTR, None, 0, None]
+    good = [PTR, PTR, PTR, 4, 32, 16, PTR, PTR, None, 0, None, 0, None]
     for at, value in ((0, None), (1, None), (2, None), (3, 0), (3, -1), (4, 0), (5, -1), (6, None), (7, None),
                       (9, 3), (9, -1)):
         args = list(good)

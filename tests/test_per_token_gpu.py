@@ -95,6 +95,34 @@ def test_mm_matches_64_bits(ops, shape, out_type, with_bias):
     assert ops.status() == 0
 
 
+@pytest.mark.parametrize("path", [1, 2, 3, 4])
+@pytest.mark.parametrize("shape", [(1, 16, 16), (1, 17, 15), (15, 300, 1300), (40, 528, 400), (65, 67, 31),
+                                   (129, 511, 1025), (256, 512, 1024), (300, 1001, 640), (600, 272, 2047),
+                                   (513, 2000, 129)])
+@pytest.mark.parametrize("out_type", [F16, BF16, F32])
+def test_mm_paths_agree(ops, path, shape, out_type):
+    """Each path (SIMT, streaming, gathering, CTA pairs) on shapes that the choice would not send it."""
+    from texo_b200 import _lib
+
+    M, N, K = shape
+    t = dtype(out_type)
+    A, B, sa, sb, bias = mm_inputs(M, N, K, sum(shape), full_range=True)
+    if t == torch.float16:
+        sa *= 0.1
+    ops.mm_int8_per_token(A[:1], B, sa[:1], sb)  # the device's set-up
+    lib = _lib.load()
+    lib.texo_mm_int8_per_token_force_path(path)
+    try:
+        got = ops.mm_int8_per_token(A, B, sa, sb, bias, out_dtype=t)
+        assert lib.texo_mm_int8_per_token_last_path() == path
+    finally:
+        lib.texo_mm_int8_per_token_force_path(0)
+    want, bound = mm_expected(A, B, sa, sb, bias, t)
+    assert_within(got, want, bound)
+    assert torch.equal(got, ops.mm_int8_per_token(A, B, sa, sb, bias, out_dtype=t))
+    assert ops.status() == 0
+
+
 @pytest.mark.parametrize("shape", [(20, 256, 8192), (160, 512, 30000), (3, 100, 4099)])
 def test_mm_extreme_values(ops, shape):
     """All -128 against all -128: the largest dots there are (2^14 K), and their rounding to FP32."""

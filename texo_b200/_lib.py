@@ -59,7 +59,8 @@ _SIGNATURES = {
     "texo_mm_int8_solve_presummed": (None, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_float, _c_float,
                                             _c_float, _c_int, _c_int, _c_int]),
     "texo_mm_int8_solve_per_token": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_ptr, _c_ptr,
-                                              _c_ptr, _c_int, _c_ptr]),
+                                              _c_ptr, _c_int, _c_ptr, ctypes.c_longlong, _c_ptr]),
+    "texo_mm_int8_per_token_workspace": (ctypes.c_longlong, [_c_ptr, _c_ptr, _c_int, _c_int, _c_int]),
     "texo_mm_int8_per_token_last_path": (_c_int, []),
     "texo_mm_int8_per_token_force_path": (None, [_c_int]),
     "texo_block_norm_solve": (_c_int, [_c_ptr] * 7 + [_c_int] * 4 + [_c_float] * 2 + [_c_int] * 3 + [_c_ptr]),

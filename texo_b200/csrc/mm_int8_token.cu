@@ -130,53 +130,105 @@ __global__ void __launch_bounds__(G_THREADS)
 // the narrow one, so an accumulator lane is an output column.
 //
 // A tile (256 columns x R rows) is worked on by a cluster of c CTAs, each on its own part of K.
-// There is no workspace: every CTA pushes its int32 partials straight into the shared memory of
-// the CTA that finishes the row (row r of a 32-row chunk belongs to CTA r % c), an mbarrier
-// there counts the pushes, and the owner adds the c copies, scales and stores.  Integer sums, so
-// the split changes no bit, and nothing is shared between calls: any streams, any graphs.
+// There is no workspace: once all of them are through, every CTA pushes its int32 partials
+// straight into the shared memory (the ring, idle by then) of the CTA that finishes the row, row
+// r going to CTA r % c; an mbarrier there counts the pushes, and the owner adds the c copies,
+// scales and stores.  Integer sums, so the split changes no bit, and nothing is shared between
+// calls: any streams, any graphs.  With c = 1 the lanes, each one output column, scale and store
+// from registers while the ring fills for the next tile.
 //
 // Shared memory is nearly all ring: an SM has to keep about 100 KiB in flight to cover HBM
 // latency at its share of the bandwidth.
 //
-// GATHER: rows of A or B that do not start at 16-byte boundaries cannot be moved by TMA.  Eight
-// or sixteen warps then build the same swizzled tiles: aligned 4-byte words, coalesced over the
-// lanes, shifted into place with their neighbour's word.
+// GATHER: rows of A or B that do not start at 16-byte boundaries cannot be moved by a tensor map.
+// Four warps then copy the 16-byte granules that hold a tile's part of each row into a raw ring
+// (cp.async; untiled bulk copies, one per row, measured 75 clocks each, four times what HBM
+// allows), and eight shift them into the swizzled tiles that the MMAs read.
 constexpr int S_BK = 128;                // k per ring stage = one 128-byte swizzle row
 constexpr int S_BOX = 128 * 128;         // 128 k rows x 128 columns of B
 constexpr int S_W_BYTES = 2 * S_BOX;     // the two boxes of a tile
 constexpr int S_TILE_N = 256;
-constexpr int S_MAX_STAGES = 6;
+constexpr int S_MAX_STAGES = 6, S_MAX_RAW_STAGES = 4;
 constexpr int S_EPI_WARPS = 8;
-constexpr int S_GATHER_GROUPS = 2, S_GATHER_WARPS = 8;  // stages are dealt to the groups in turn
+constexpr int S_GATHER_GROUPS = 2, S_GATHER_WARPS = 4;  // stages are dealt to the groups in turn
+constexpr int S_COPY_WARPS = 4;                         // warp 0 and the last three
 constexpr int S_THREADS = 64 + S_EPI_WARPS * 32;
-constexpr int S_GATHER_THREADS = S_THREADS + S_GATHER_GROUPS * S_GATHER_WARPS * 32;
+constexpr int S_GATHER_THREADS = S_THREADS + (S_GATHER_GROUPS * S_GATHER_WARPS + S_COPY_WARPS - 1) * 32;
 constexpr int S_MAX_CLUSTER = 8;
 
-__host__ __device__ constexpr int s_chunk_rows(int R) { return R < 32 ? R : 32; }
-// Rows of a chunk that one CTA of the cluster finishes.
-__host__ __device__ constexpr int s_slots(int R, int c) { return (s_chunk_rows(R) + c - 1) / c; }
-__host__ __device__ constexpr int s_stages(int R) { return R == 16 ? 6 : R == 32 ? 5 : 4; }
-__host__ __device__ constexpr int s_stage_bytes(int R) { return S_W_BYTES + R * 128; }
-__host__ __device__ constexpr int s_push_bytes(int R, int c) { return c * s_slots(R, c) * S_TILE_N * 4; }
-__host__ __device__ constexpr int s_smem_bytes(int R, int c) {
-  return s_stages(R) * s_stage_bytes(R) + s_push_bytes(R, c) + 1024 /*alignment*/ + 256 /*barriers*/;
+__host__ __device__ constexpr int s_stages(int R, bool gather) {
+  return gather ? 2 : R <= 32 ? 6 : R == 64 ? 5 : 4;
 }
-static_assert(s_smem_bytes(128, 8) <= 232448 && s_smem_bytes(64, 7) <= 232448 && s_smem_bytes(32, 7) <= 232448 &&
-                  s_smem_bytes(16, 7) <= 232448 && s_smem_bytes(16, 5) <= 232448,
+__host__ __device__ constexpr int s_stage_bytes(int R) { return S_W_BYTES + R * 128; }
+// Raw ring: the granules that hold 256 bytes of each k row of B, at any offset, and 128 of each
+// row of A.
+constexpr int S_RAW_B_ROW = 256 + 16, S_RAW_A_ROW = 128 + 16;
+__host__ __device__ constexpr int s_raw_bytes(int R) { return S_BK * S_RAW_B_ROW + R * S_RAW_A_ROW; }
+__host__ __device__ constexpr int s_raw_stages(int R) { return R == 16 ? 4 : R == 128 ? 2 : 3; }
+__host__ __device__ constexpr int s_ring_bytes(int R, bool gather) {
+  return s_stages(R, gather) * s_stage_bytes(R) + (gather ? s_raw_stages(R) * s_raw_bytes(R) : 0);
+}
+__host__ __device__ constexpr int s_smem_bytes(int R, bool gather) {
+  return s_ring_bytes(R, gather) + 1024 /*alignment*/ + 256 /*barriers*/;
+}
+// Rows of a tile that one CTA of the cluster finishes, and the room that their partials take.
+__host__ __device__ constexpr int s_slots(int R, int c) { return (R + c - 1) / c; }
+__host__ __device__ constexpr int s_push_bytes(int R, int c) { return c * s_slots(R, c) * S_TILE_N * 4; }
+constexpr int SMEM_LIMIT = 232448;
+__host__ __device__ constexpr bool s_fits(int R, bool gather) {
+  return s_smem_bytes(R, gather) <= SMEM_LIMIT && s_push_bytes(R, 7) <= s_ring_bytes(R, gather) &&
+         s_push_bytes(R, 6) <= s_ring_bytes(R, gather) && s_push_bytes(R, 5) <= s_ring_bytes(R, gather) &&
+         s_push_bytes(R, 3) <= s_ring_bytes(R, gather) && s_push_bytes(R, 8) <= s_ring_bytes(R, gather);
+}
+static_assert(s_fits(16, false) && s_fits(32, false) && s_fits(64, false) && s_fits(128, false) && s_fits(16, true) &&
+                  s_fits(32, true) && s_fits(64, true) && s_fits(128, true),
               "streaming kernel: shared memory over the limit");
 
 struct StreamBarriers {
   uint64_t full[S_MAX_STAGES];
   uint64_t empty[S_MAX_STAGES];
+  uint64_t raw_full[S_MAX_RAW_STAGES];   // GATHER: a k block's granules have landed
+  uint64_t raw_empty[S_MAX_RAW_STAGES];  // and have been shifted into place
   uint64_t acc_full[2];
   uint64_t acc_empty[2];
-  uint64_t pushed;  // all partials of a chunk have arrived in this CTA
-  uint64_t taken;   // all CTAs have finished reading a chunk's partials
+  uint64_t ring_idle;  // c > 1: every CTA of the cluster is through with its part of K
+  uint64_t pushed;     // all partials of a tile have arrived in this CTA
+  uint64_t taken;      // and have been read: the ring may fill again
   uint32_t tmem_base;
   int abort_flag;
 };
 static_assert(sizeof(StreamBarriers) <= 256, "StreamBarriers outgrew its shared-memory reserve");
 
+// Shared-memory accesses by address: the aligned base of the ring is computed from integers, so
+// the compiler would take accesses through its pointer for generic ones (measured 4 times as
+// slow in the shifting warps).
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ unsigned short lds16(uint32_t addr) {
+  unsigned short v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ int4 lds128(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ void sts64(uint32_t addr, uint32_t x, uint32_t y) {
+  asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(addr), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void sts128(uint32_t addr, float x, float y, float z, float w) {
+  asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(x), "f"(y), "f"(z), "f"(w) : "memory");
+}
 __device__ __forceinline__ void store_cluster_u32(uint32_t cluster_addr, uint32_t v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
 }
@@ -191,14 +243,158 @@ __device__ __forceinline__ void drain_loads(uint64_t* full, int stages, int issu
   }
 }
 
-// The aligned word at p, of which bytes outside [begin, end) are not read and come back as 0.
-__device__ __forceinline__ uint32_t load_word(const uint8_t* p, const uint8_t* begin, const uint8_t* end) {
-  if (p >= begin && p + 4 <= end) return __ldg(reinterpret_cast<const unsigned int*>(p));
-  uint32_t v = 0;
+// A whole warp's wait.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status,
+                                          int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, code));
+}
+__device__ __forceinline__ bool warp_wait_cluster(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                                  int* status, int code) {
+  return __all_sync(0xffffffffu, mbar_wait_cluster(bar, parity, abort_flag, status, code));
+}
+
+// Whether the phase has completed, without waiting for it.
+__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// Sixteen bytes global -> shared, asynchronously and past L1; both addresses aligned.
+__device__ __forceinline__ void copy_granule(uint32_t dst, uintptr_t src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All but this thread's N last groups of copies have landed.
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uintptr_t floor16(uintptr_t a) { return a & ~uintptr_t(15); }
+__device__ __forceinline__ uintptr_t ceil16(uintptr_t a) { return (a + 15) & ~uintptr_t(15); }
+
+// The gathering form's view of a row-major operand: where a block of it starts and how far its
+// rows are apart.  Rows that are sixteen apart start at the same offset in their granule
+// (sixteen pitches are a multiple of sixteen bytes), so a thread that keeps to one row of
+// sixteen works with constant offsets.
+struct Block {
+  uintptr_t corner;  // first byte of the block
+  int pitch, rows;
+  uintptr_t begin, end;  // of the operand
+  __device__ uintptr_t row(int r) const { return corner + size_t(r) * pitch; }
+  // Whether `bytes` from the granule of each row's first byte on lie in the operand: for a block
+  // whose every row has that, or row by row.
+  __device__ bool inside(int bytes) const {
+    return corner - 15 >= begin && row(rows - 1) + bytes <= end;
+  }
+  __device__ bool row_inside(int r, int bytes) const {
+    return floor16(row(r)) >= begin && floor16(row(r)) + bytes <= end;
+  }
+};
+
+// Copies GRANULES + 1 granules from each row's first byte on, to (GRANULES + 1) * 16 apart in
+// shared memory.  Thread t of S_COPY_WARPS * 32: granule t % GRANULES of every (threads /
+// GRANULES)th row, then the last granule of row t.  What reaches outside the operand is left out
+// (edge_word reads that).
+template <int GRANULES>
+__device__ __forceinline__ void copy_rows(uint32_t smem_dst, const Block& b, int t) {
+  constexpr int ROWS = S_COPY_WARPS * 32 / GRANULES, ROW_BYTES = (GRANULES + 1) * 16;
+  static_assert(16 % ROWS == 0 && S_COPY_WARPS * 32 >= 128, "a thread keeps to a few rows of sixteen");
+  const int g = t % GRANULES;
+  const size_t step = 16 * size_t(b.pitch);
+  const bool inside = b.inside(ROW_BYTES);
 #pragma unroll
+  for (int part = 0; part < 16 / ROWS; ++part) {
+    const int r0 = t / GRANULES + part * ROWS;
+    uint32_t dst = smem_dst + r0 * ROW_BYTES + g * 16;
+    uintptr_t from = floor16(b.row(r0)) + g * 16;
+    if (inside) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (r0 + i * 16 < b.rows) copy_granule(dst + i * 16 * ROW_BYTES, from);
+        from += step;
+      }
+    } else {
+      for (int r = r0; r < b.rows; r += 16, from += step, dst += 16 * ROW_BYTES)
+        if (from >= b.begin && from + 16 <= b.end) copy_granule(dst, from);
+    }
+  }
+  if (t < b.rows) {
+    const uintptr_t last = floor16(b.row(t)) + GRANULES * 16;
+    if (inside || (last >= b.begin && last + 16 <= b.end))
+      copy_granule(smem_dst + t * ROW_BYTES + GRANULES * 16, last);
+  }
+}
+
+// Word `w` from a row's first granule on, which is `granules` in shared memory and at address
+// `from`; where its granule reaches outside the operand its bytes come from memory.
+__device__ __noinline__ uint32_t edge_word(uint32_t granules, uintptr_t from, int w, uintptr_t begin,
+                                           uintptr_t end) {
+  const uintptr_t granule = from + w / 4 * 16, at = from + w * 4;
+  if (granule >= begin && granule + 16 <= end) return lds32(granules + w * 4);
+  uint32_t v = 0;
   for (int e = 0; e < 4; ++e)
-    if (p + e >= begin && p + e < end) v |= uint32_t(p[e]) << (8 * e);
+    if (at + e >= begin && at + e < end) v |= uint32_t(*reinterpret_cast<const uint8_t*>(at + e)) << (8 * e);
   return v;
+}
+
+// Shifts WORDS * 4 bytes (WORDS: 32 or 64) of each row of a block from their granules into
+// 128-byte rows with the swizzle of the MMA's operands, the second 32 words S_BOX further on.
+// A warp's share: the rows whose number mod 16 is within [OWN gw, OWN gw + OWN); a lane moves one
+// word (or two) of each: two conflict-free loads, a funnel shift, a conflict-free store; four
+// rows' loads before the first store.  `mask` keeps a lane's bytes that the rows still have.
+template <int WORDS>
+__device__ __forceinline__ void shift_rows(uint32_t to, uint32_t granules, const Block& b, int gw, int lane,
+                                           uint32_t mask) {
+  constexpr int ROW_BYTES = WORDS * 4 + 16, BOXES = WORDS / 32, OWN = 16 / S_GATHER_WARPS;
+  const int sixteens = (b.rows + 15) / 16;  // (the ring has room for whole sixteens)
+#pragma unroll
+  for (int j = 0; j < OWN; ++j) {
+    const int r0 = gw * OWN + j;
+    const unsigned offset = unsigned(b.row(r0)) & 15, bits = (offset & 3) * 8;
+    const uint32_t from = granules + r0 * ROW_BYTES + (offset & 12) + lane * 4;
+    const uint32_t dst = to + r0 * 128 + (((lane / 4) ^ (r0 & 7)) << 4) + lane % 4 * 4;
+#pragma unroll
+    for (int i0 = 0; i0 < 8; i0 += 4) {
+      if (i0 >= sixteens) break;
+      uint32_t v[4][BOXES];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int h = 0; h < BOXES; ++h) {
+          const uint32_t w = from + (i0 + i) * 16 * ROW_BYTES + h * 128;
+          v[i][h] = i0 + i < sixteens ? __funnelshift_r(lds32(w), lds32(w + 4), bits) & mask : 0u;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (r0 + (i0 + i) * 16 < b.rows) {  // warp-uniform
+#pragma unroll
+          for (int h = 0; h < BOXES; ++h) sts32(dst + (i0 + i) * 16 * 128 + h * S_BOX, v[i][h]);
+        }
+      }
+    }
+  }
+  if (!b.inside(ROW_BYTES)) {  // once more for the rows at the operand's first and last bytes
+    for (int r = gw * OWN; r < b.rows; r += (r % OWN == OWN - 1 ? 17 - OWN : 1)) {
+      if (b.row_inside(r, ROW_BYTES)) continue;
+      const unsigned offset = unsigned(b.row(r)) & 15;
+      const uint32_t from = granules + r * ROW_BYTES;
+      const uintptr_t first = floor16(b.row(r));
+      for (int h = 0; h < BOXES; ++h) {
+        const int w = h * 32 + lane + offset / 4;
+        sts32(to + h * S_BOX + r * 128 + (((lane / 4) ^ (r & 7)) << 4) + lane % 4 * 4,
+              __funnelshift_r(edge_word(from, first, w, b.begin, b.end), edge_word(from, first, w + 1, b.begin, b.end),
+                              (offset & 3) * 8) & mask);
+      }
+    }
+  }
 }
 
 struct StreamShape {
@@ -216,9 +412,11 @@ __global__ void __launch_bounds__(GATHER ? S_GATHER_THREADS : S_THREADS, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   grid_dependency_trigger();
   const int R = p.R, c = p.cluster;
-  const int stages = s_stages(R), stage_bytes = s_stage_bytes(R);
-  uint32_t* push = reinterpret_cast<uint32_t*>(smem + stages * stage_bytes);
-  StreamBarriers* bars = reinterpret_cast<StreamBarriers*>(smem + stages * stage_bytes + s_push_bytes(R, c));
+  const int stages = s_stages(R, GATHER), stage_bytes = s_stage_bytes(R);
+  const uint32_t push = smem_u32(smem);  // c > 1: partials, over the idle ring
+  uint8_t* raw = smem + stages * stage_bytes;
+  const int raw_stages = s_raw_stages(R), raw_bytes = s_raw_bytes(R);
+  StreamBarriers* bars = reinterpret_cast<StreamBarriers*>(smem + s_ring_bytes(R, GATHER));
   volatile int* abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int rank = int(cluster_ctarank());
@@ -232,12 +430,17 @@ __global__ void __launch_bounds__(GATHER ? S_GATHER_THREADS : S_THREADS, 1)
       mbar_init(&bars->full[i], GATHER ? S_GATHER_WARPS : 1);
       mbar_init(&bars->empty[i], 1);
     }
+    for (int i = 0; GATHER && i < raw_stages; ++i) {
+      mbar_init(&bars->raw_full[i], S_COPY_WARPS);
+      mbar_init(&bars->raw_empty[i], S_GATHER_WARPS);
+    }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&bars->acc_full[b], 1);
       mbar_init(&bars->acc_empty[b], S_EPI_WARPS);
     }
+    mbar_init(&bars->ring_idle, c);
     mbar_init(&bars->pushed, c * S_EPI_WARPS);
-    mbar_init(&bars->taken, c * S_EPI_WARPS);
+    mbar_init(&bars->taken, S_EPI_WARPS);
     bars->abort_flag = 0;
     fence_barrier_init();
     if (!GATHER) {
@@ -260,15 +463,76 @@ __global__ void __launch_bounds__(GATHER ? S_GATHER_THREADS : S_THREADS, 1)
   tc_fence_after_sync();
   const uint32_t tmem_base = bars->tmem_base;
 
-  if (warp == 0) {
+  constexpr int FIRST_COPY_WARP = 2 + S_EPI_WARPS + S_GATHER_GROUPS * S_GATHER_WARPS;
+  if (GATHER && (warp == 0 || warp >= FIRST_COPY_WARP)) {
+    // ---------------------------------------------------------------- granules
+    const int t = warp == 0 ? lane : (warp - FIRST_COPY_WARP + 1) * 32 + lane;
+    const uintptr_t a_begin = reinterpret_cast<uintptr_t>(A), a_end = a_begin + size_t(p.M) * p.K;
+    const uintptr_t b_begin = reinterpret_cast<uintptr_t>(B), b_end = b_begin + size_t(p.K) * p.N;
+    int stage = 0, pending = 0, done = 0;  // k blocks under way; stage of the oldest of them
+    uint32_t phase = 0, taken_phase = 0;
+    bool ok = true;
+    auto landed = [&]() {  // this thread's copies have landed: the warp's oldest block is complete
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->raw_full[done]);
+      if (++done == raw_stages) done = 0;
+      --pending;
+    };
+    auto all_landed = [&]() {
+      wait_copies<0>();
+      while (pending > 0) landed();
+    };
+    grid_dependency_wait();
+    for (int tile = first_tile; tile < p.tiles && ok; tile += tile_step) {
+      const int n0 = tile / p.m_tiles * S_TILE_N, m0 = tile % p.m_tiles * R;
+      const int rows = min(R, p.M - m0);
+      if (c > 1 && tile != first_tile) {
+        ok = warp_wait(&bars->taken, taken_phase, abort_flag, status, STATUS_TIMEOUT_FLAG);
+        if (!ok) break;
+        taken_phase ^= 1;
+      }
+      for (int kb = kb0; kb < kb1; ++kb) {
+        // before the warp waits for room it hands over what it has
+        int room = 1;
+        if (lane == 0) room = mbar_test_wait(&bars->raw_empty[stage], phase ^ 1);
+        if (!__shfl_sync(0xffffffffu, room, 0)) {
+          all_landed();
+          ok = warp_wait(&bars->raw_empty[stage], phase ^ 1, abort_flag, status, STATUS_TIMEOUT_EMPTY);
+          if (!ok) break;
+        }
+        const uint32_t block = smem_u32(raw) + stage * raw_bytes;
+        const int k0 = kb * S_BK;
+        const Block block_b = {b_begin + size_t(k0) * p.N + n0, p.N, min(S_BK, p.K - k0), b_begin, b_end};
+        const Block block_a = {a_begin + size_t(m0) * p.K + k0, p.K, rows, a_begin, a_end};
+        copy_rows<16>(block, block_b, t);
+        copy_rows<8>(block + S_BK * S_RAW_B_ROW, block_a, t);
+        commit_copies();
+        if (++pending == 3) {
+          wait_copies<2>();
+          landed();
+        }
+        if (++stage == raw_stages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+      all_landed();
+    }
+    wait_copies<0>();
+  } else if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
-    if (!GATHER && lane == 0) {
+    if (lane == 0) {
       int stage = 0, issued = 0;
-      uint32_t phase = 0;
+      uint32_t phase = 0, taken_phase = 0;
       bool ok = true;
       grid_dependency_wait();  // the operands may have been written by the grid ahead
       for (int tile = first_tile; tile < p.tiles && ok; tile += tile_step) {
         const int n0 = tile / p.m_tiles * S_TILE_N, m0 = tile % p.m_tiles * R;
+        if (c > 1 && tile != first_tile) {
+          ok = mbar_wait(&bars->taken, taken_phase, abort_flag, status, STATUS_TIMEOUT_FLAG);
+          if (!ok) break;
+          taken_phase ^= 1;
+        }
         for (int kb = kb0; kb < kb1; ++kb) {
           ok = mbar_wait(&bars->empty[stage], phase ^ 1, abort_flag, status, STATUS_TIMEOUT_EMPTY);
           if (!ok) break;
@@ -328,73 +592,79 @@ __global__ void __launch_bounds__(GATHER ? S_GATHER_THREADS : S_THREADS, 1)
   } else if (warp < 2 + S_EPI_WARPS) {
     // ---------------------------------------------------------------- epilogue
     const int ew = warp - 2, quarter = warp % 4, half = ew / 4;
-    const int column = half * 128 + quarter * 32 + lane;
-    const int chunk_rows = s_chunk_rows(R), slots = s_slots(R, c);
-    const uint32_t push_addr = smem_u32(push);
-    int buf = 0, chunk_no = 0;
-    uint32_t buf_phase = 0;
+    const int column = half * 128 + quarter * 32 + lane;  // of the tile
+    int buf = 0;
+    uint32_t buf_phase = 0, tile_phase = 0;
     bool ok = true;
     grid_dependency_wait();  // before the scales are read and the output is written
     for (int tile = first_tile; tile < p.tiles && ok; tile += tile_step) {
       const int n0 = tile / p.m_tiles * S_TILE_N, m0 = tile % p.m_tiles * R;
       const int rows = min(R, p.M - m0);
-      ok = mbar_wait(&bars->acc_full[buf], buf_phase, abort_flag, status, STATUS_TIMEOUT_TMEM_FULL);
-      ok = __all_sync(0xffffffffu, ok);
+      ok = warp_wait(&bars->acc_full[buf], buf_phase, abort_flag, status, STATUS_TIMEOUT_TMEM_FULL);
       if (!ok) break;
       tc_fence_after_sync();
-      for (int r0 = 0; r0 < rows; r0 += chunk_rows, ++chunk_no) {
-        const int here = min(chunk_rows, rows - r0);
-        uint32_t v[32];
-        const uint32_t at = tmem_base + (buf * 2 + half) * R + r0 + (uint32_t(quarter * 32) << 16);
-        if (R == 16) {
-          uint32_t v16[16];
-          tmem_ld_32x16(at, v16);
+      const uint32_t acc = tmem_base + (buf * 2 + half) * R + (uint32_t(quarter * 32) << 16);
+      if (c == 1) {
+        const int n = n0 + column;
+        const bool in = n < p.N;
+        const float sb = in ? __ldg(s.b + n) : 0.f, bias = in && s.bias ? __ldg(s.bias + n) : 0.f;
+        Y* column_out = out + size_t(m0) * p.N + n;
+        for (int r0 = 0; r0 < rows; r0 += 16) {
+          uint32_t v[16];
+          tmem_ld_32x16(acc + r0, v);
+          const int m = min(m0 + r0 + lane % 16, p.M - 1);
+          const float sa_lane = __ldg(s.a + m);
           tmem_ld_wait();
 #pragma unroll
-          for (int r = 0; r < 16; ++r) v[r] = v16[r];
-        } else {
-          tmem_ld_32x32(at, v);
+          for (int r = 0; r < 16; ++r) {
+            const float sa = __shfl_sync(0xffffffffu, sa_lane, r);
+            if (in && r0 + r < rows)
+              column_out[size_t(r0 + r) * p.N] = row::from_float<Y>(scaled(float(int(v[r])), sa, sb, bias));
+          }
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->acc_empty[buf]);
+      } else {
+        // all of this CTA's loads have landed and all its MMAs have read them
+        if (ew == 0 && lane < c) mbar_arrive_cluster(map_to_cta(smem_u32(&bars->ring_idle), lane));
+        ok = warp_wait_cluster(&bars->ring_idle, tile_phase, abort_flag, status, STATUS_TIMEOUT_FLAG);
+        if (!ok) break;
+        const int slots = s_slots(R, c);
+        const uint32_t to = push + uint32_t((rank * slots * S_TILE_N + column) * 4);
+        int owner = 0;
+        uint32_t slot_bytes = 0;
+        for (int r0 = 0; r0 < rows; r0 += 16) {
+          uint32_t v[16];
+          tmem_ld_32x16(acc + r0, v);
           tmem_ld_wait();
-        }
-        if (r0 + chunk_rows >= rows) {  // the accumulator is in registers: its buffer is free
-          tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars->acc_empty[buf]);
-        }
-        if (chunk_no > 0) {  // the last chunk's partials have been read everywhere
-          ok = mbar_wait_cluster(&bars->taken, (chunk_no - 1) & 1, abort_flag, status, STATUS_TIMEOUT_FLAG);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-        }
-        {
-          int owner = 0, slot = 0;
 #pragma unroll
-          for (int r = 0; r < 32; ++r) {
-            if (r < here) {
-              store_cluster_u32(map_to_cta(push_addr, owner) + uint32_t(((rank * slots + slot) * S_TILE_N + column) * 4),
-                                v[r]);
+          for (int r = 0; r < 16; ++r) {
+            if (r0 + r < rows) {
+              store_cluster_u32(map_to_cta(to + slot_bytes, owner), v[r]);
               if (++owner == c) {
                 owner = 0;
-                ++slot;
+                slot_bytes += S_TILE_N * 4;
               }
             }
           }
         }
+        tc_fence_before_sync();
         __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->acc_empty[buf]);
         if (lane < c) mbar_arrive_cluster(map_to_cta(smem_u32(&bars->pushed), lane));
-        ok = mbar_wait_cluster(&bars->pushed, chunk_no & 1, abort_flag, status, STATUS_TIMEOUT_FLAG);
-        ok = __all_sync(0xffffffffu, ok);
+        ok = warp_wait_cluster(&bars->pushed, tile_phase, abort_flag, status, STATUS_TIMEOUT_FLAG);
         if (!ok) break;
-        for (int slot = ew; slot * c + rank < here; slot += S_EPI_WARPS) {
-          const int m = m0 + r0 + slot * c + rank;
-          const uint32_t* first = push + slot * S_TILE_N;
+        for (int slot = ew; slot * c + rank < rows; slot += S_EPI_WARPS) {
+          const int m = m0 + slot * c + rank;
+          const uint32_t first = push + slot * S_TILE_N * 4;
           const float sa = __ldg(s.a + m);
           Y* row_out = out + size_t(m) * p.N + n0;
           if (p.vector_out && n0 + lane * 8 + 8 <= p.N) {
             int total[8] = {};
             for (int copy = 0; copy < c; ++copy) {
-              const int4* w = reinterpret_cast<const int4*>(first + copy * slots * S_TILE_N + lane * 8);
-              const int4 lo = w[0], hi = w[1];
+              const uint32_t w = first + (copy * slots * S_TILE_N + lane * 8) * 4;
+              const int4 lo = lds128(w), hi = lds128(w + 16);
               total[0] += lo.x, total[1] += lo.y, total[2] += lo.z, total[3] += lo.w;
               total[4] += hi.x, total[5] += hi.y, total[6] += hi.z, total[7] += hi.w;
             }
@@ -406,19 +676,24 @@ __global__ void __launch_bounds__(GATHER ? S_GATHER_THREADS : S_THREADS, 1)
             }
             row::store8(row_out + lane * 8, y);
           } else if (!p.vector_out) {
-#pragma unroll 1
+            int total[8] = {};
+            for (int copy = 0; copy < c; ++copy) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) total[j] += int(lds32(first + (copy * slots * S_TILE_N + j * 32 + lane) * 4));
+            }
+#pragma unroll
             for (int j = 0; j < 8; ++j) {
-              const int n = j * 32 + lane;
-              if (n0 + n >= p.N) break;
-              int total = 0;
-              for (int copy = 0; copy < c; ++copy) total += int(first[copy * slots * S_TILE_N + n]);
-              row_out[n] = row::from_float<Y>(
-                  scaled(float(total), sa, __ldg(s.b + n0 + n), s.bias ? __ldg(s.bias + n0 + n) : 0.f));
+              const int n = n0 + j * 32 + lane;
+              if (n < p.N)
+                row_out[j * 32 + lane] = row::from_float<Y>(
+                    scaled(float(total[j]), sa, __ldg(s.b + n), s.bias ? __ldg(s.bias + n) : 0.f));
             }
           }
         }
+        fence_proxy_async_smem();  // these accesses come before the loads that fill the ring again
         __syncwarp();
-        if (lane < c) mbar_arrive_cluster(map_to_cta(smem_u32(&bars->taken), lane));
+        if (lane == 0) mbar_arrive(&bars->taken);
+        tile_phase ^= 1;
       }
       if (++buf == 2) {
         buf = 0;
@@ -426,71 +701,48 @@ __global__ void __launch_bounds__(GATHER ? S_GATHER_THREADS : S_THREADS, 1)
       }
     }
   } else {
-    // ------------------------------------------------------------------ gather
+    // ----------------------------------------------------------------- shifting
     const int group = (warp - 2 - S_EPI_WARPS) / S_GATHER_WARPS, gw = (warp - 2 - S_EPI_WARPS) % S_GATHER_WARPS;
-    const uint8_t *a_begin = reinterpret_cast<const uint8_t*>(A), *a_end = a_begin + size_t(p.M) * p.K;
-    const uint8_t *b_begin = reinterpret_cast<const uint8_t*>(B), *b_end = b_begin + size_t(p.K) * p.N;
-    int stage = 0, turn = 0;
-    uint32_t phase = 0;
+    const uintptr_t a_begin = reinterpret_cast<uintptr_t>(A), a_end = a_begin + size_t(p.M) * p.K;
+    const uintptr_t b_begin = reinterpret_cast<uintptr_t>(B), b_end = b_begin + size_t(p.K) * p.N;
+    int stage = 0, raw_stage = 0, turn = 0;
+    uint32_t phase = 0, raw_phase = 0;
     bool ok = true;
     grid_dependency_wait();
     for (int tile = first_tile; tile < p.tiles && ok; tile += tile_step) {
       const int n0 = tile / p.m_tiles * S_TILE_N, m0 = tile % p.m_tiles * R;
+      const int rows = min(R, p.M - m0);
       for (int kb = kb0; kb < kb1 && ok; ++kb) {
         if (turn == group) {
-          constexpr int ROWS = S_BK / S_GATHER_WARPS;
-          // this lane's words of sixteen k rows: bytes 4 * lane .. of either box
-          uint32_t w[ROWS][2], tail[ROWS];
-#pragma unroll
-          for (int i = 0; i < ROWS; ++i) {
-            const int k = kb * S_BK + gw + i * S_GATHER_WARPS;
-            w[i][0] = w[i][1] = tail[i] = 0;
-            if (k < p.K) {
-              const uint8_t* src = b_begin + size_t(k) * p.N + n0;
-              const uint8_t* word = src - (reinterpret_cast<uintptr_t>(src) & 3);
-              w[i][0] = load_word(word + lane * 4, b_begin, b_end);
-              w[i][1] = load_word(word + 128 + lane * 4, b_begin, b_end);
-              if (lane == 31) tail[i] = load_word(word + 256, b_begin, b_end);
-            }
-          }
-          ok = mbar_wait(&bars->empty[stage], phase ^ 1, abort_flag, status, STATUS_TIMEOUT_EMPTY);
-          ok = __all_sync(0xffffffffu, ok);
+          ok = warp_wait(&bars->empty[stage], phase ^ 1, abort_flag, status, STATUS_TIMEOUT_EMPTY) &&
+               warp_wait(&bars->raw_full[raw_stage], raw_phase, abort_flag, status, STATUS_TIMEOUT_FULL);
           if (!ok) break;
-          uint8_t* sw = smem + stage * stage_bytes;
-#pragma unroll
-          for (int i = 0; i < ROWS; ++i) {
-            const int kr = gw + i * S_GATHER_WARPS;
-            const unsigned shift = unsigned((reinterpret_cast<uintptr_t>(b_begin) + size_t(kb * S_BK + kr) * p.N + n0) & 3) * 8;
-            // the word after this lane's: its neighbour's, or the next box's first, or the tail
-            const uint32_t next0 = __shfl_sync(0xffffffffu, lane == 0 ? w[i][1] : w[i][0], (lane + 1) & 31);
-            const uint32_t next1 = __shfl_sync(0xffffffffu, w[i][1], (lane + 1) & 31);
-            const uint32_t v0 = __funnelshift_r(w[i][0], next0, shift);
-            const uint32_t v1 = __funnelshift_r(w[i][1], lane == 31 ? tail[i] : next1, shift);
-            const int at = kr * 128 + (((lane / 4) ^ (kr & 7)) << 4) + (lane % 4) * 4;
-            *reinterpret_cast<uint32_t*>(sw + at) = v0;
-            *reinterpret_cast<uint32_t*>(sw + S_BOX + at) = v1;
-          }
-          // activations: k of the row past K must be zero (what it meets in B is arbitrary)
-          for (int r = gw; r < R && m0 + r < p.M; r += S_GATHER_WARPS) {
-            const uint8_t* src = a_begin + size_t(m0 + r) * p.K + size_t(kb) * S_BK;
-            const unsigned mis = unsigned(reinterpret_cast<uintptr_t>(src) & 3);
-            const uint8_t* word = src - mis;
-            const uint32_t mine = load_word(word + lane * 4, a_begin, a_end);
-            uint32_t next = __shfl_down_sync(0xffffffffu, mine, 1);
-            if (lane == 31) next = load_word(word + 128, a_begin, a_end);
-            uint32_t v = __funnelshift_r(mine, next, mis * 8);
-            const int left = p.K - (kb * S_BK + lane * 4);
-            if (left < 4) v = left <= 0 ? 0u : v & ((1u << (8 * left)) - 1);
-            *reinterpret_cast<uint32_t*>(sw + S_W_BYTES + r * 128 + (((lane / 4) ^ (r & 7)) << 4) + (lane % 4) * 4) = v;
-          }
+          const uint32_t sw = smem_u32(smem) + stage * stage_bytes;
+          const uint32_t block = smem_u32(raw) + raw_stage * raw_bytes;
+          const int k0 = kb * S_BK;
+          // What a tile of B holds past K, or past the last column, meets a zero of A or goes to no
+          // output; A's bytes past K have to be zero.
+          const Block block_b = {b_begin + size_t(k0) * p.N + n0, p.N, min(S_BK, p.K - k0), b_begin, b_end};
+          const Block block_a = {a_begin + size_t(m0) * p.K + k0, p.K, rows, a_begin, a_end};
+          const int left = p.K - k0 - lane * 4;
+          shift_rows<64>(sw, block, block_b, gw, lane, 0xffffffffu);
+          shift_rows<32>(sw + S_W_BYTES, block + S_BK * S_RAW_B_ROW, block_a, gw, lane,
+                         left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1);
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bars->full[stage]);
+          if (lane == 0) {
+            mbar_arrive(&bars->full[stage]);
+            mbar_arrive(&bars->raw_empty[raw_stage]);
+          }
         }
         if (++turn == S_GATHER_GROUPS) turn = 0;
         if (++stage == stages) {
           stage = 0;
           phase ^= 1;
+        }
+        if (++raw_stage == raw_stages) {
+          raw_stage = 0;
+          raw_phase ^= 1;
         }
       }
     }
@@ -517,7 +769,7 @@ constexpr int P_EPI_WARPS = 8;
 constexpr int P_THREADS = 64 + P_EPI_WARPS * 32;
 constexpr int P_OUT_BYTES = 32 * 128;  // a warp's staging tile
 constexpr int P_SMEM_BYTES = P_STAGES * P_STAGE_BYTES + P_EPI_WARPS * P_OUT_BYTES + 1024 + 256;
-static_assert(P_SMEM_BYTES <= 232448, "pair kernel: shared memory over the limit");
+static_assert(P_SMEM_BYTES <= SMEM_LIMIT, "pair kernel: shared memory over the limit");
 
 struct PairBarriers {
   uint64_t full[P_STAGES];  // even CTA: both CTAs' bytes
@@ -546,10 +798,12 @@ struct PairShape {
   int M, N, K, tiles_m, tiles_n, raster_rows;
 };
 
-template <typename Y>
+// TMA_OUT: rows of Y start at 16-byte boundaries, and the scales' at theirs.  Otherwise a warp
+// reads its staging tile back row by row and stores element by element.
+template <typename Y, bool TMA_OUT>
 __global__ void __launch_bounds__(P_THREADS, 1)
     pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                const __grid_constant__ CUtensorMap map_y, Scales s, PairShape p, int* status) {
+                const __grid_constant__ CUtensorMap map_y, Y* __restrict__ out, Scales s, PairShape p, int* status) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   grid_dependency_trigger();
@@ -573,7 +827,7 @@ __global__ void __launch_bounds__(P_THREADS, 1)
     fence_barrier_init();
     tma_prefetch_desc(&map_a);
     tma_prefetch_desc(&map_b);
-    tma_prefetch_desc(&map_y);
+    if (TMA_OUT) tma_prefetch_desc(&map_y);
   }
   if (warp == 1) {
     tmem_alloc_pair(&bars->tmem_base, 512);
@@ -655,7 +909,7 @@ __global__ void __launch_bounds__(P_THREADS, 1)
     constexpr int COLS = 128 / int(sizeof(Y));  // columns of a staging tile
     const int ew = warp - 2, quarter = warp % 4, half = ew / 4;
     uint8_t* stage_out = staging + ew * P_OUT_BYTES;
-    uint8_t* my_row = stage_out + lane * 128;
+    const uint32_t my_row = smem_u32(stage_out) + lane * 128;
     int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
@@ -666,14 +920,13 @@ __global__ void __launch_bounds__(P_THREADS, 1)
       const int m0 = tm * 256 + rank * 128 + quarter * 32;  // this warp's first row
       const int n0 = tn * 256 + half * 128;                 // and column
       const float sa = m0 + lane < p.M ? __ldg(s.a + m0 + lane) : 0.f;
-      ok = mbar_wait(&bars->acc_full[acc], acc_phase, abort_flag, status, STATUS_TIMEOUT_TMEM_FULL);
-      ok = __all_sync(0xffffffffu, ok);
+      ok = warp_wait(&bars->acc_full[acc], acc_phase, abort_flag, status, STATUS_TIMEOUT_TMEM_FULL);
       if (!ok) break;
       tc_fence_after_sync();
 #pragma unroll 1
       for (int col = 0; col < 128; col += COLS) {
         if (m0 >= p.M || n0 + col >= p.N) break;  // warp-uniform
-        if (lane == 0) tma_store_wait_read<0>();  // the last store has read the staging tile
+        if (TMA_OUT && lane == 0) tma_store_wait_read<0>();  // the last store has read the staging tile
         __syncwarp();
 #pragma unroll
         for (int sub = 0; sub < COLS; sub += 32) {
@@ -683,29 +936,56 @@ __global__ void __launch_bounds__(P_THREADS, 1)
           const int n = n0 + col + sub;
 #pragma unroll
           for (int g = 0; g < 8; ++g) {
-            // N is a multiple of 16 here: four columns are inside or outside as a whole
             float4 sb = make_float4(0.f, 0.f, 0.f, 0.f), bias = sb;
-            if (n + g * 4 < p.N) {
-              sb = __ldg(reinterpret_cast<const float4*>(s.b + n + g * 4));
-              if (s.bias) bias = __ldg(reinterpret_cast<const float4*>(s.bias + n + g * 4));
+            if (TMA_OUT) {  // N is a multiple of 16: four columns are inside or outside as a whole
+              if (n + g * 4 < p.N) {
+                sb = __ldg(reinterpret_cast<const float4*>(s.b + n + g * 4));
+                if (s.bias) bias = __ldg(reinterpret_cast<const float4*>(s.bias + n + g * 4));
+              }
+            } else {
+              float* sb_of = &sb.x;
+              float* bias_of = &bias.x;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int at = min(n + g * 4 + e, p.N - 1);
+                sb_of[e] = __ldg(s.b + at);
+                if (s.bias) bias_of[e] = __ldg(s.bias + at);
+              }
             }
             const float y0 = scaled(float(int(v[g * 4])), sa, sb.x, bias.x);
             const float y1 = scaled(float(int(v[g * 4 + 1])), sa, sb.y, bias.y);
             const float y2 = scaled(float(int(v[g * 4 + 2])), sa, sb.z, bias.z);
             const float y3 = scaled(float(int(v[g * 4 + 3])), sa, sb.w, bias.w);
             if constexpr (sizeof(Y) == 4) {
-              *reinterpret_cast<float4*>(my_row + ((g ^ (lane & 7)) << 4)) = make_float4(y0, y1, y2, y3);
+              sts128(my_row + ((g ^ (lane & 7)) << 4), y0, y1, y2, y3);
             } else {
-              *reinterpret_cast<uint2*>(my_row + (((sub / 8 + g / 2) ^ (lane & 7)) << 4) + (g & 1) * 8) =
-                  make_uint2(pack2<Y>(y0, y1), pack2<Y>(y2, y3));
+              sts64(my_row + (((sub / 8 + g / 2) ^ (lane & 7)) << 4) + (g & 1) * 8, pack2<Y>(y0, y1), pack2<Y>(y2, y3));
             }
           }
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          tma_store_2d(&map_y, stage_out, n0 + col, m0);  // rows and columns outside Y are dropped
-          tma_store_commit();
+        if (TMA_OUT) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&map_y, stage_out, n0 + col, m0);  // rows and columns outside Y are dropped
+            tma_store_commit();
+          }
+        } else {
+          __syncwarp();
+          const int rows = min(32, p.M - m0);
+          for (int r = 0; r < rows; ++r) {
+#pragma unroll
+            for (int sub = 0; sub < COLS; sub += 32) {
+              const int n = n0 + col + sub + lane, byte = (sub + lane) * int(sizeof(Y));
+              const uint32_t at = smem_u32(stage_out) + r * 128 + (((byte / 16) ^ (r & 7)) << 4) + byte % 16;
+              if (n < p.N) {
+                if constexpr (sizeof(Y) == 4)
+                  out[size_t(m0 + r) * p.N + n] = __uint_as_float(lds32(at));
+                else
+                  reinterpret_cast<unsigned short*>(out)[size_t(m0 + r) * p.N + n] = lds16(at);
+              }
+            }
+          }
         }
       }
       tc_fence_before_sync();
@@ -716,7 +996,7 @@ __global__ void __launch_bounds__(P_THREADS, 1)
         acc_phase ^= 1;
       }
     }
-    if (lane == 0) tma_store_wait_all<0>();
+    if (TMA_OUT && lane == 0) tma_store_wait_all<0>();
   }
 
   tc_fence_before_sync();
@@ -725,6 +1005,60 @@ __global__ void __launch_bounds__(P_THREADS, 1)
   if (warp == 1) {
     tc_fence_after_sync();
     tmem_dealloc_pair(tmem_base, 512);
+  }
+}
+
+// ------------------------------------------------------------------- padding
+// Copies of A and B whose rows start at 16-byte boundaries, in the caller's workspace: what the
+// gathering kernel does per tile, once per call.  Rows of `width` bytes become rows of `pitch`
+// (the next multiple of 16) bytes; the bytes between are arbitrary (tensor maps end at `width`).
+// A warp moves 512 bytes of a row: four coalesced words per lane, shifted into place with the
+// word that follows.
+struct Pad {
+  const uint8_t* from;
+  uint8_t* to;
+  long long rows;
+  int width, pitch;
+  long long pieces() const { return rows * ((pitch + 511) / 512); }
+};
+constexpr int PAD_THREADS = 256;
+__global__ void __launch_bounds__(PAD_THREADS) pad_kernel(const Pad a, const Pad b, long long a_pieces,
+                                                          long long pieces) {
+  grid_dependency_trigger();
+  grid_dependency_wait();
+  const int lane = threadIdx.x % 32;
+  for (long long i = (long long)blockIdx.x * (PAD_THREADS / 32) + threadIdx.x / 32; i < pieces;
+       i += (long long)gridDim.x * (PAD_THREADS / 32)) {
+    const Pad& p = i < a_pieces ? a : b;
+    const long long piece = i < a_pieces ? i : i - a_pieces;
+    const int per_row = (p.pitch + 511) / 512;
+    const long long row = piece / per_row;
+    const int c0 = int(piece % per_row) * 512 + lane * 4;
+    const uintptr_t begin = reinterpret_cast<uintptr_t>(p.from), end = begin + size_t(p.rows) * p.width;
+    const uintptr_t src = begin + size_t(row) * p.width + c0;
+    const uintptr_t word = src & ~uintptr_t(3);
+    const unsigned bits = unsigned(src & 3) * 8;
+    uint32_t w[4][2];
+    if (word >= begin && word + 3 * 128 + 8 <= end) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        w[j][0] = __ldg(reinterpret_cast<const unsigned int*>(word + j * 128));
+        w[j][1] = __ldg(reinterpret_cast<const unsigned int*>(word + j * 128 + 4));
+      }
+    } else {
+      for (int j = 0; j < 4; ++j)
+        for (int h = 0; h < 2; ++h) {
+          w[j][h] = 0;
+          for (int e = 0; e < 4; ++e) {
+            const uintptr_t at = word + j * 128 + h * 4 + e;
+            if (at >= begin && at < end) w[j][h] |= uint32_t(*reinterpret_cast<const uint8_t*>(at)) << (8 * e);
+          }
+        }
+    }
+    uint32_t* to = reinterpret_cast<uint32_t*>(p.to + size_t(row) * p.pitch + c0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (c0 + j * 128 < p.pitch) to[j * 32] = __funnelshift_r(w[j][0], w[j][1], bits);
   }
 }
 
@@ -811,9 +1145,10 @@ struct DeviceSetup {
 static DeviceSetup setups[MAX_DEVICES];
 template <typename Y>
 static void configure_kernels() {
-  cudaFuncSetAttribute(stream_kernel<Y, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
-  cudaFuncSetAttribute(stream_kernel<Y, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
-  cudaFuncSetAttribute(pair_kernel<Y>, cudaFuncAttributeMaxDynamicSharedMemorySize, P_SMEM_BYTES);
+  cudaFuncSetAttribute(stream_kernel<Y, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
+  cudaFuncSetAttribute(stream_kernel<Y, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
+  cudaFuncSetAttribute(pair_kernel<Y, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, P_SMEM_BYTES);
+  cudaFuncSetAttribute(pair_kernel<Y, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, P_SMEM_BYTES);
 }
 static DeviceSetup& device_setup(DeviceCtx& ctx) {
   DeviceSetup& d = setups[ctx.device];
@@ -823,22 +1158,28 @@ static DeviceSetup& device_setup(DeviceCtx& ctx) {
     configure_kernels<float>();
     for (int r = 0; r < 4; ++r) {
       for (int c = 1; c <= S_MAX_CLUSTER; ++c) {
-        const int R = R_CHOICES[r], bytes = s_smem_bytes(R, c);
-        if (bytes > 232448) continue;
-        d.clusters[0][r][c] = max_clusters(stream_kernel<__half, false>, S_THREADS, bytes, c);
-        d.clusters[1][r][c] = max_clusters(stream_kernel<__half, true>, S_GATHER_THREADS, bytes, c);
+        const int R = R_CHOICES[r];
+        d.clusters[0][r][c] = max_clusters(stream_kernel<__half, false>, S_THREADS, s_smem_bytes(R, false), c);
+        d.clusters[1][r][c] = max_clusters(stream_kernel<__half, true>, S_GATHER_THREADS, s_smem_bytes(R, true), c);
       }
     }
-    d.pairs = max_clusters(pair_kernel<__half>, P_THREADS, P_SMEM_BYTES, 2);
+    d.pairs = max_clusters(pair_kernel<__half, true>, P_THREADS, P_SMEM_BYTES, 2);
     cudaGetLastError();
     d.ready = true;
   }
   return d;
 }
 
+// The choice between the paths is by estimated time in microseconds.  The constants are fits to
+// measurements on B200 (kernels back to back, operands from HBM):
+//   stream, per k block of 128: 0.42 + 0.0009 R, or its 32 KiB of B at 6.2 TB/s over all CTAs
+//   gather, per k block: 1.15 up to R = 32, then 1.4 (64) and 1.9 (128): shared-memory bandwidth
+//   either, per call: 3.2 (c = 1) or 4.7, and 0.045 R for the drain
+//   pair, per k block 0.33 (0.42 once all SMs run: power), per call 7, per round of tiles 1
+//   padding: 2.5 and twice the operand's bytes at 5 TB/s
 struct StreamPlan {
   int R = 0, cluster = 0, clusters = 0, m_tiles = 0, tiles = 0;
-  double us = 1e30;  // estimate
+  double us = 1e30;
 };
 static StreamPlan plan_stream(const DeviceSetup& d, bool gather, int M, int N, int K) {
   StreamPlan best;
@@ -852,74 +1193,137 @@ static StreamPlan plan_stream(const DeviceSetup& d, bool gather, int M, int N, i
     if (held <= 0) continue;
     const int clusters = int(std::min<long long>(tiles, held));
     const double rounds = double((tiles + clusters - 1) / clusters);
-    const double kb = (num_kb + c - 1) / c;
-    const double rate = std::min(58e3, 6.4e6 / (clusters * c));  // bytes per us and SM
-    const double us = rounds * (kb * s_stage_bytes(R) / rate + 1.0 + 0.3 * (c > 1) + 0.01 * R) + 3;
+    const double block = gather ? (R <= 32 ? 1.15 : R == 64 ? 1.4 : 1.9)
+                                : std::max(0.42 + 0.0009 * R, 32768.0 * clusters * c / double(m_tiles) / 6.2e6);
+    const double us = rounds * ((num_kb + c - 1) / c * block + (c > 1 ? 2 : 0.3)) + (c > 1 ? 2.7 : 2.9) + 0.045 * R;
     if (us < best.us) best = {R, c, clusters, int(m_tiles), int(tiles), us};
   }
   return best;
 }
 
+struct Route {
+  int path = PATH_GENERIC;
+  bool pad_a = false, pad_b = false;
+  StreamPlan stream;
+  double us = 1e30;
+};
+static int padded(int width) { return (width + 15) & ~15; }
+static long long pad_bytes(int M, int N, int K, bool a, bool b) {
+  return (a ? (long long)M * padded(K) : 0) + (b ? (long long)K * padded(N) : 0);
+}
+// a_ok / b_ok: TMA can move the operand as it lies.
+static Route choose_route(const DeviceSetup& d, int M, int N, int K, bool a_ok, bool b_ok, long long workspace,
+                          int force) {
+  Route best;
+  if (K <= 0 || K >= (1 << 17) || force == PATH_GENERIC) return best;
+  const long long pad = pad_bytes(M, N, K, !a_ok, !b_ok);
+  if (pad <= workspace && force != PATH_STREAM_GATHER) {
+    const double pad_us = pad ? 2.5 + 2.0 * double(pad) / 5e6 : 0;
+    if (force != PATH_PAIR) {
+      const StreamPlan plan = plan_stream(d, false, M, N, K);
+      if (plan.cluster > 0) best = {PATH_STREAM, !a_ok, !b_ok, plan, plan.us + pad_us};
+    }
+    const long long tiles = (long long)((M + 255) / 256) * ((N + 255) / 256);
+    if (d.pairs > 0 && tiles <= 0x3fffffff && force != PATH_STREAM) {
+      const double rounds = double((tiles + d.pairs - 1) / d.pairs);
+      const double us = 7 + rounds * ((K + 127) / 128 * (rounds > 2 ? 0.42 : 0.33) + 1) + pad_us;
+      if (us < best.us) best = {PATH_PAIR, !a_ok, !b_ok, StreamPlan(), us};
+    }
+  }
+  if (force == PATH_STREAM_GATHER || (force == PATH_AUTO && pad > 0) || best.us > 1e29) {
+    const StreamPlan plan = plan_stream(d, true, M, N, K);
+    if (plan.cluster > 0 && plan.us < best.us) best = {PATH_STREAM_GATHER, false, false, plan, plan.us};
+  }
+  return best;
+}
+
+// An operand as a kernel gets it: its rows and how far they are apart.
+struct Operand {
+  const int8_t* p;
+  int pitch;
+};
+
 template <typename Y, bool GATHER>
-static bool launch_stream(DeviceCtx& ctx, const StreamPlan& plan, const int8_t* A, const int8_t* B, Y* out, int M,
+static bool launch_stream(DeviceCtx& ctx, const StreamPlan& plan, const Operand& A, const Operand& B, Y* out, int M,
                           int N, int K, const Scales& s, cudaStream_t stream) {
   CUtensorMap map_b = {}, map_a = {};
-  if (!GATHER && (!make_tensor_map_2d(&map_b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, B, K, N, N, S_BK, 128,
+  if (!GATHER && (!make_tensor_map_2d(&map_b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, B.p, K, N, B.pitch, S_BK, 128,
                                       CU_TENSOR_MAP_SWIZZLE_128B) ||
-                  !make_tensor_map_2d(&map_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, A, M, K, K, plan.R, S_BK,
+                  !make_tensor_map_2d(&map_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, A.p, M, K, A.pitch, plan.R, S_BK,
                                       CU_TENSOR_MAP_SWIZZLE_128B)))
     return false;
   const StreamShape p = {M, N, K, plan.R, plan.cluster, plan.m_tiles, plan.tiles,
                          N % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0};
-  last_path() = GATHER ? PATH_STREAM_GATHER : PATH_STREAM;
   return launch_clusters(stream_kernel<Y, GATHER>, plan.clusters * plan.cluster,
-                         GATHER ? S_GATHER_THREADS : S_THREADS, s_smem_bytes(plan.R, plan.cluster), plan.cluster,
-                         stream, map_b, map_a, A, B, out, s, p, ctx.status);
+                         GATHER ? S_GATHER_THREADS : S_THREADS, s_smem_bytes(plan.R, GATHER), plan.cluster, stream,
+                         map_b, map_a, A.p, B.p, out, s, p, ctx.status);
 }
 
 template <typename Y>
-static bool launch_pair(DeviceCtx& ctx, const DeviceSetup& d, const int8_t* A, const int8_t* B, Y* out, int M, int N,
-                        int K, const Scales& s, cudaStream_t stream) {
-  CUtensorMap map_a, map_b, map_y;
+static bool launch_pair(DeviceCtx& ctx, const DeviceSetup& d, const Operand& A, const Operand& B, Y* out, int M,
+                        int N, int K, const Scales& s, cudaStream_t stream) {
+  CUtensorMap map_a, map_b, map_y = {};
   constexpr CUtensorMapDataType TYPE = std::is_same<Y, float>::value    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                        : std::is_same<Y, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                                         : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  if (!make_tensor_map_2d(&map_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, A, M, K, K, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B) ||
-      !make_tensor_map_2d(&map_b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, B, K, N, N, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B) ||
-      !make_tensor_map_2d(&map_y, TYPE, sizeof(Y), out, M, N, size_t(N) * sizeof(Y), 32, 128 / sizeof(Y),
-                          CU_TENSOR_MAP_SWIZZLE_128B))
+  auto aligned = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+  const bool tma_out = N % 16 == 0 && aligned(out) && aligned(s.b) && aligned(s.bias);
+  if (!make_tensor_map_2d(&map_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, A.p, M, K, A.pitch, 128, 128,
+                          CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !make_tensor_map_2d(&map_b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, B.p, K, N, B.pitch, 128, 128,
+                          CU_TENSOR_MAP_SWIZZLE_128B) ||
+      (tma_out && !make_tensor_map_2d(&map_y, TYPE, sizeof(Y), out, M, N, size_t(N) * sizeof(Y), 32, 128 / sizeof(Y),
+                                      CU_TENSOR_MAP_SWIZZLE_128B)))
     return false;
   const PairShape p = {M, N, K, (M + 255) / 256, (N + 255) / 256, i8::raster_group_rows(K)};
   const int clusters = std::min(p.tiles_m * p.tiles_n, d.pairs);
-  last_path() = PATH_PAIR;
-  return launch_clusters(pair_kernel<Y>, 2 * clusters, P_THREADS, P_SMEM_BYTES, 2, stream, map_a, map_b, map_y, s, p,
-                         ctx.status);
+  return tma_out ? launch_clusters(pair_kernel<Y, true>, 2 * clusters, P_THREADS, P_SMEM_BYTES, 2, stream, map_a,
+                                   map_b, map_y, out, s, p, ctx.status)
+                 : launch_clusters(pair_kernel<Y, false>, 2 * clusters, P_THREADS, P_SMEM_BYTES, 2, stream, map_a,
+                                   map_b, map_y, out, s, p, ctx.status);
+}
+
+// Makes the padded copies in the workspace and points the operands at them.
+static bool launch_pad(const DeviceCtx& ctx, const Route& route, Operand& A, Operand& B, int M, int N, int K,
+                       void* workspace, cudaStream_t stream) {
+  uint8_t* to = static_cast<uint8_t*>(workspace);
+  Pad a = {}, b = {};
+  if (route.pad_a) {
+    a = {reinterpret_cast<const uint8_t*>(A.p), to, M, K, padded(K)};
+    A = {reinterpret_cast<int8_t*>(to), padded(K)};
+    to += size_t(M) * padded(K);
+  }
+  if (route.pad_b) {
+    b = {reinterpret_cast<const uint8_t*>(B.p), to, K, N, padded(N)};
+    B = {reinterpret_cast<int8_t*>(to), padded(N)};
+  }
+  const long long a_pieces = a.pieces(), pieces = a_pieces + b.pieces();
+  const int grid = int(std::min<long long>((pieces + PAD_THREADS / 32 - 1) / (PAD_THREADS / 32), ctx.sm_count * 8));
+  return launch_clusters(pad_kernel, grid, PAD_THREADS, 0, 1, stream, a, b, a_pieces, pieces);
+}
+
+static bool tma_can_move(const int8_t* p, int width) {
+  return width % 16 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 }
 
 template <typename Y>
-static int solve(const int8_t* A, const int8_t* B, Y* out, int M, int N, int K, const Scales& s,
-                 cudaStream_t stream) {
-  auto aligned = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+static int solve(const int8_t* A, const int8_t* B, Y* out, int M, int N, int K, const Scales& s, void* workspace,
+                 long long workspace_bytes, cudaStream_t stream) {
   int device;
   if ((!device_ctx_entry(device).ready || !setups[device].ready) && is_capturing(stream)) return -4;
   DeviceCtx& ctx = device_ctx();
   const DeviceSetup& d = device_setup(ctx);
-  const int force = forced_path();
-  if (ctx.cc_major >= 10 && K > 0 && K < (1 << 17) && force != PATH_GENERIC) {
-    const bool tma = K % 16 == 0 && N % 16 == 0 && aligned(A) && aligned(B);
-    const bool pair_ok = tma && d.pairs > 0 && aligned(out) && aligned(s.b) && aligned(s.bias) &&
-                         (long long)((M + 255) / 256) * ((N + 255) / 256) <= 0x3fffffff;
-    const StreamPlan plan = plan_stream(d, !tma || force == PATH_STREAM_GATHER, M, N, K);
-    if (pair_ok && force != PATH_STREAM && force != PATH_STREAM_GATHER) {
-      const double rounds = ((long long)((M + 255) / 256) * ((N + 255) / 256) + d.pairs - 1) / d.pairs;
-      const double us = 6 + rounds * (0.3 * ((K + 127) / 128) + 1);
-      if ((force == PATH_PAIR || us < plan.us) && launch_pair(ctx, d, A, B, out, M, N, K, s, stream)) return 0;
-    }
-    if (plan.cluster > 0) {
-      const bool gather = !tma || force == PATH_STREAM_GATHER;
-      if (gather ? launch_stream<Y, true>(ctx, plan, A, B, out, M, N, K, s, stream)
-                 : launch_stream<Y, false>(ctx, plan, A, B, out, M, N, K, s, stream))
-        return 0;
+  if (ctx.cc_major >= 10) {
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0) workspace_bytes = 0;
+    const Route route = choose_route(d, M, N, K, tma_can_move(A, K), tma_can_move(B, N), workspace_bytes, forced_path());
+    Operand a = {A, K}, b = {B, N};
+    if (route.path != PATH_GENERIC &&
+        (!(route.pad_a || route.pad_b) || launch_pad(ctx, route, a, b, M, N, K, workspace, stream)) &&
+        (route.path == PATH_PAIR     ? launch_pair(ctx, d, a, b, out, M, N, K, s, stream)
+         : route.path == PATH_STREAM ? launch_stream<Y, false>(ctx, route.stream, a, b, out, M, N, K, s, stream)
+                                     : launch_stream<Y, true>(ctx, route.stream, a, b, out, M, N, K, s, stream))) {
+      last_path() = route.path;
+      return 0;
     }
   }
   if (!launch_generic(A, B, out, M, N, K, s, stream)) {
@@ -932,17 +1336,31 @@ static int solve(const int8_t* A, const int8_t* B, Y* out, int M, int N, int K, 
 }  // namespace i8t
 }  // namespace texo
 
+extern "C" long long texo_mm_int8_per_token_workspace(const int8_t* A, const int8_t* B, int M, int N, int K) {
+  using namespace texo;
+  const bool a_ok = i8t::tma_can_move(A, K), b_ok = i8t::tma_can_move(B, N);
+  int device;
+  if (M <= 0 || N <= 0 || K <= 0 || (a_ok && b_ok) || !device_ctx_entry(device).ready || !i8t::setups[device].ready)
+    return 0;
+  const i8t::Route route =
+      i8t::choose_route(i8t::setups[device], M, N, K, a_ok, b_ok, 0x7fffffffffffffffLL, i8t::forced_path());
+  return i8t::pad_bytes(M, N, K, route.pad_a, route.pad_b);
+}
+
 extern "C" int texo_mm_int8_solve_per_token(const int8_t* A, const int8_t* B, void* Y, int M, int N, int K,
                                             const float* scale_A, const float* scale_B, const float* bias,
-                                            int out_type, void* stream) {
+                                            int out_type, void* workspace, long long workspace_bytes, void* stream) {
   using namespace texo;
   if (M <= 0 || N <= 0 || K < 0 || !Y || !scale_A || !scale_B || (K > 0 && (!A || !B))) return -1;
   const i8t::Scales s = {scale_A, scale_B, bias};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (out_type) {
-    case row::TYPE_F16: return i8t::solve(A, B, static_cast<__half*>(Y), M, N, K, s, st);
-    case row::TYPE_BF16: return i8t::solve(A, B, static_cast<__nv_bfloat16*>(Y), M, N, K, s, st);
-    case row::TYPE_F32: return i8t::solve(A, B, static_cast<float*>(Y), M, N, K, s, st);
+    case row::TYPE_F16:
+      return i8t::solve(A, B, static_cast<__half*>(Y), M, N, K, s, workspace, workspace_bytes, st);
+    case row::TYPE_BF16:
+      return i8t::solve(A, B, static_cast<__nv_bfloat16*>(Y), M, N, K, s, workspace, workspace_bytes, st);
+    case row::TYPE_F32:
+      return i8t::solve(A, B, static_cast<float*>(Y), M, N, K, s, workspace, workspace_bytes, st);
     default: return -1;
   }
 }

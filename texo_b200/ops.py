@@ -528,9 +528,15 @@ def mm_int8_per_token(A: torch.Tensor, B: torch.Tensor, scale_A: torch.Tensor, s
         raise ValueError(f"out_dtype must be float16, bfloat16 or float32, got {out_dtype}")
     out = _check_out("out", out, (M, N), out_dtype, A)
     if M > 0:
-        _call_on_stream("texo_mm_int8_solve_per_token", A, (B, scale_A, scale_B, bias, out),
-                        A.data_ptr() if K else None, B.data_ptr() if K else None, out.data_ptr(), M, N, K,
-                        scale_A.data_ptr(), scale_B.data_ptr(), _ptr(bias), code)
+        a, b = (A.data_ptr(), B.data_ptr()) if K else (None, None)
+        workspace, size = None, 0
+        if K % 16 or N % 16 or (K and (a | b) % 16):  # operands that TMA cannot move may be copied
+            with torch.cuda.device(A.device):
+                size = _lib.load().texo_mm_int8_per_token_workspace(a, b, M, N, K)
+            if size:
+                workspace = torch.empty(size, dtype=torch.uint8, device=A.device)
+        _call_on_stream("texo_mm_int8_solve_per_token", A, (B, scale_A, scale_B, bias, out), a, b, out.data_ptr(),
+                        M, N, K, scale_A.data_ptr(), scale_B.data_ptr(), _ptr(bias), code, _ptr(workspace), size)
     return out
 
 
