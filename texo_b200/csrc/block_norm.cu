@@ -12,8 +12,8 @@
 // All of it in FP32.  z is rounded once, to the residual's type, on its way to memory; y is
 // computed from the unrounded z, so that a 16-bit residual stream costs y nothing.
 //
-// Bound by HBM bandwidth: a row lives in registers between the reductions (row_ops.cuh), so
-// every input byte is read once and every output byte written once.
+// Bound by HBM bandwidth: a row lives in registers between the reductions, so every input byte
+// is read once and every output byte written once (row_ops.cuh).
 #include <cstdint>
 #include <cuda_runtime.h>
 
@@ -29,118 +29,127 @@ struct Args {
   void *y, *z;
   int8_t* q;
   float* scale;
-  long long N;
-  int C;
-  long long rows_per_gate;
+  int N, C;
+  int rows_per_gate;
   int gate_per_channel;  // 0: one value per gate row
   float eps, residual_scale;
+  float inv_c;  // 1 / C
   int weights_f32;  // weight, post_weight and gate are FP32 (else they have x's type)
 };
 
-// Eight values of a weight-like row, in either of its two types.
-template <bool VECTOR, typename X>
-__device__ __forceinline__ void load_weights(const void* base, bool f32, size_t offset, int C, int thread,
-                                             int threads, int i, float (&v)[8]) {
+// Group i of a weight-like row, in either of its two types.
+template <typename X, row::Layout L>
+__device__ __forceinline__ void load_weights(const row::Spread<L>& s, const void* base, bool f32, size_t offset, int i,
+                                             float (&v)[8]) {
   if (f32)
-    row::load_shared_group<VECTOR>(static_cast<const float*>(base) + offset, C, thread, threads, i, v);
+    s.template load<false>(static_cast<const float*>(base) + offset, i, v);
   else
-    row::load_shared_group<VECTOR>(static_cast<const X*>(base) + offset, C, thread, threads, i, v);
+    s.template load<false>(static_cast<const X*>(base) + offset, i, v);
 }
 
-// The row in registers.  blockDim = (threads of a row, rows of the block).
-template <typename X, typename R, bool QUANT, bool VECTOR, int UNITS>
-__global__ void __launch_bounds__(UNITS == 4 ? 512 : 1024)
-    row_kernel(const Args a) {
-  __shared__ float sum_scratch[2][row::MAX_WARPS];
-  __shared__ unsigned max_scratch[row::MAX_WARPS];
-  const long long n = (long long)blockIdx.x * blockDim.y + threadIdx.y;
-  if (n >= a.N) return;  // only blocks of one-warp rows reach past N; they meet at no barrier
-  const int t = threadIdx.x, threads = blockDim.x, warps = threads / 32, C = a.C;
-  const size_t at = size_t(n) * C;
-  const X* x = static_cast<const X*>(a.x) + at;
-  const R* residual = static_cast<const R*>(a.residual) + at;
+template <int UNITS>
+__device__ __forceinline__ float squares(const float (&v)[UNITS][8]) {
+  float sum[8];
+  row::mul8(sum, v[0], v[0]);
+#pragma unroll
+  for (int i = 1; i < UNITS; ++i) row::fma8(sum, v[i], v[i], sum);
+  return ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
+}
 
-  row::Raw8<X> xr[UNITS];
-  row::Raw8<R> rr[UNITS];
-#pragma unroll
-  for (int i = 0; i < UNITS; ++i) xr[i] = row::load_group<VECTOR>(x, C, t, threads, i);
-#pragma unroll
-  for (int i = 0; i < UNITS; ++i) rr[i] = row::load_group<VECTOR>(residual, C, t, threads, i);
-
-  float v[UNITS][8];
-#pragma unroll
-  for (int i = 0; i < UNITS; ++i) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[i][j] = row::to_float(xr[i].v[j]);
-  }
+// x (group i) -> u: the block's own norm and the gate, whose row is `gate_row`.
+template <typename X, row::Layout L>
+__device__ __forceinline__ void to_u(const Args& a, size_t gate_row, const row::Spread<L>& s, int i, float post_inv,
+                                     float (&v)[8]) {
   if (a.post_weight) {
-    float sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < UNITS; ++i) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) sum += v[i][j] * v[i][j];
-    }
-    const float inv = rsqrtf(row::row_sum(sum, sum_scratch[0], warps) / float(C) + a.eps);
-#pragma unroll
-    for (int i = 0; i < UNITS; ++i) {
-      float w[8];
-      load_weights<VECTOR, X>(a.post_weight, a.weights_f32, 0, C, t, threads, i, w);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] *= inv * w[j];
-    }
+    float w[8];
+    load_weights<X>(s, a.post_weight, a.weights_f32, 0, i, w);
+    row::mul8(w, w, post_inv);
+    row::mul8(v, v, w);
   }
   if (a.gate) {
-    const size_t row = size_t(n / a.rows_per_gate);
     if (a.gate_per_channel) {
-#pragma unroll
-      for (int i = 0; i < UNITS; ++i) {
-        float g[8];
-        load_weights<VECTOR, X>(a.gate, a.weights_f32, row * C, C, t, threads, i, g);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] *= g[j];
-      }
+      float g[8];
+      load_weights<X>(s, a.gate, a.weights_f32, gate_row * a.C, i, g);
+      row::mul8(v, v, g);
     } else {
-      const float g = a.weights_f32 ? static_cast<const float*>(a.gate)[row]
-                                    : row::to_float(static_cast<const X*>(a.gate)[row]);
-#pragma unroll
-      for (int i = 0; i < UNITS; ++i) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] *= g;
-      }
+      const float g = a.weights_f32 ? static_cast<const float*>(a.gate)[gate_row]
+                                    : row::to_float(static_cast<const X*>(a.gate)[gate_row]);
+      row::mul8(v, v, g);
     }
   }
-  float sum = 0.f;
-  R* z = static_cast<R*>(a.z) + at;
-#pragma unroll
-  for (int i = 0; i < UNITS; ++i) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      // values past the row's end are products with a zero: not for a gate that is infinite or NaN
-      const bool in = row::position<VECTOR>(t, threads, i, j) < C;
-      v[i][j] = in ? __fmaf_rn(a.residual_scale, row::to_float(rr[i].v[j]), v[i][j]) : 0.f;
-      sum += v[i][j] * v[i][j];
-    }
-    row::store_group<VECTOR>(z, C, t, threads, i, v[i]);
-  }
-  const float inv = rsqrtf(row::row_sum(sum, sum_scratch[1], warps) / float(C) + a.eps);
-  unsigned amax = 0;
+}
+
+// u and the residual (group i) -> z, in registers and to memory.  Values past the row's end become
+// zero whatever they were.
+template <typename R, row::Layout L>
+__device__ __forceinline__ void to_z(const Args& a, int n, const row::Spread<L>& s, int i, const float (&r)[8],
+                                     float (&v)[8]) {
+  row::fma8(v, r, a.residual_scale, v);
+  s.mask(i, v);
+  s.store(static_cast<R*>(a.z) + size_t(n) * a.C, i, v);
+}
+
+// z -> the outputs.
+template <typename X, bool QUANT, row::Layout L, int UNITS>
+__device__ __forceinline__ void finish(const Args& a, int n, const row::Spread<L>& s, float (&v)[UNITS][8],
+                                       float* sum_scratch, unsigned* max_scratch) {
+  const int warps = s.threads / 32;
+  const float inv = rsqrtf(row::row_sum(squares(v), sum_scratch, s.t, warps) * a.inv_c + a.eps);
+  const size_t at = size_t(n) * a.C;
+  float amax = 0.f;
 #pragma unroll
   for (int i = 0; i < UNITS; ++i) {
     float w[8];
-    load_weights<VECTOR, X>(a.weight, a.weights_f32, 0, C, t, threads, i, w);
+    load_weights<X>(s, a.weight, a.weights_f32, 0, i, w);
+    row::mul8(w, w, inv);
+    row::mul8(v[i], v[i], w);
+    if (QUANT) {
+      s.mask(i, v[i]);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      v[i][j] *= inv * w[j];
-      if (QUANT && row::position<VECTOR>(t, threads, i, j) < C) amax = max(amax, __float_as_uint(fabsf(v[i][j])));
+      for (int j = 0; j < 8; ++j) amax = row::max_abs(amax, v[i][j]);
+    } else {
+      s.store(static_cast<X*>(a.y) + at, i, v[i]);
     }
-    if (!QUANT) row::store_group<VECTOR>(static_cast<X*>(a.y) + at, C, t, threads, i, v[i]);
   }
   if (QUANT) {
-    const row::TokenScale s = row::token_scale(row::row_max(amax, max_scratch, warps));
-    if (t == 0) a.scale[n] = s.scale;
+    amax = row::row_max(amax, max_scratch, s.t, warps);
+    if (s.t == 0) a.scale[n] = row::token_scale(amax);
+    const float inverse = row::token_inverse(amax);
 #pragma unroll
-    for (int i = 0; i < UNITS; ++i) row::store_quantised<VECTOR>(a.q + at, C, t, threads, i, v[i], s.inverse);
+    for (int i = 0; i < UNITS; ++i) s.store_quantised(a.q + at, i, v[i], inverse);
   }
+}
+
+struct Scratch {
+  float post[row::MAX_WARPS], sum[row::MAX_WARPS];
+  unsigned max[row::MAX_WARPS];
+};
+
+// A block (or a warp) per row.  blockDim = (threads of a row, rows of the block).
+template <typename X, typename R, bool QUANT, row::Layout L, int UNITS>
+__global__ void __launch_bounds__(1024) row_kernel(const Args a) {
+  __shared__ Scratch scratch;
+  grid_dependency_trigger();
+  const long long row_number = (long long)blockIdx.x * blockDim.y + threadIdx.y;
+  if (row_number >= a.N) return;  // only blocks of one-warp rows reach past N; they meet at no barrier
+  const int n = int(row_number);
+  const row::Spread<L> s = {int(threadIdx.x), int(blockDim.x), a.C};
+  const size_t gate_row = a.gate ? size_t(unsigned(n) / unsigned(a.rows_per_gate)) : 0;
+  grid_dependency_wait();
+  float v[UNITS][8], r[UNITS][8];
+#pragma unroll
+  for (int i = 0; i < UNITS; ++i) s.template load<true>(static_cast<const X*>(a.x) + size_t(n) * a.C, i, v[i]);
+#pragma unroll
+  for (int i = 0; i < UNITS; ++i) s.template load<true>(static_cast<const R*>(a.residual) + size_t(n) * a.C, i, r[i]);
+  float post_inv = 1.f;
+  if (a.post_weight)
+    post_inv = rsqrtf(row::row_sum(squares(v), scratch.post, s.t, s.threads / 32) * a.inv_c + a.eps);
+#pragma unroll
+  for (int i = 0; i < UNITS; ++i) {
+    to_u<X>(a, gate_row, s, i, post_inv, v[i]);
+    to_z<R>(a, n, s, i, r[i], v[i]);
+  }
+  finish<X, QUANT>(a, n, s, v, scratch.sum, scratch.max);
 }
 
 // Rows that the registers do not hold: the values are computed again from x and residual in
@@ -149,10 +158,11 @@ __global__ void __launch_bounds__(UNITS == 4 ? 512 : 1024)
 constexpr int LONG_THREADS = 1024;
 template <typename X, typename R, bool QUANT>
 __global__ void __launch_bounds__(LONG_THREADS) long_row_kernel(const Args a) {
-  __shared__ float sum_scratch[2][row::MAX_WARPS];
-  __shared__ unsigned max_scratch[row::MAX_WARPS];
+  __shared__ Scratch scratch;
+  grid_dependency_trigger();
+  grid_dependency_wait();
   constexpr int WARPS = LONG_THREADS / 32;
-  const long long n = blockIdx.x;
+  const int n = blockIdx.x;
   const int C = a.C;
   const size_t at = size_t(n) * C;
   const X* x = static_cast<const X*>(a.x) + at;
@@ -167,9 +177,9 @@ __global__ void __launch_bounds__(LONG_THREADS) long_row_kernel(const Args a) {
       const float v = row::to_float(x[c]);
       sum += v * v;
     }
-    post_inv = rsqrtf(row::row_sum(sum, sum_scratch[0], WARPS) / float(C) + a.eps);
+    post_inv = rsqrtf(row::row_sum(sum, scratch.post, threadIdx.x, WARPS) / float(C) + a.eps);
   }
-  const size_t gate_row = a.gate ? size_t(n / a.rows_per_gate) : 0;
+  const size_t gate_row = a.gate ? size_t(unsigned(n) / unsigned(a.rows_per_gate)) : 0;
   auto z_at = [&](int c) {
     float v = row::to_float(x[c]);
     if (a.post_weight) v *= post_inv * weight(a.post_weight, c);
@@ -181,75 +191,63 @@ __global__ void __launch_bounds__(LONG_THREADS) long_row_kernel(const Args a) {
     const float v = z_at(c);
     sum += v * v;
   }
-  const float inv = rsqrtf(row::row_sum(sum, sum_scratch[1], WARPS) / float(C) + a.eps);
-  row::TokenScale s = {0.f, 0.f};
+  const float inv = rsqrtf(row::row_sum(sum, scratch.sum, threadIdx.x, WARPS) / float(C) + a.eps);
+  float inverse = 0.f;
   if (QUANT) {
-    unsigned amax = 0;
-    for (int c = threadIdx.x; c < C; c += LONG_THREADS)
-      amax = max(amax, __float_as_uint(fabsf(z_at(c) * (inv * weight(a.weight, c)))));
-    s = row::token_scale(row::row_max(amax, max_scratch, WARPS));
-    if (threadIdx.x == 0) a.scale[n] = s.scale;
+    float amax = 0.f;
+    for (int c = threadIdx.x; c < C; c += LONG_THREADS) amax = row::max_abs(amax, z_at(c) * (inv * weight(a.weight, c)));
+    amax = row::row_max(amax, scratch.max, threadIdx.x, WARPS);
+    if (threadIdx.x == 0) a.scale[n] = row::token_scale(amax);
+    inverse = row::token_inverse(amax);
   }
   for (int c = threadIdx.x; c < C; c += LONG_THREADS) {
     const float z = z_at(c);
     const float y = z * (inv * weight(a.weight, c));
     static_cast<R*>(a.z)[at + c] = row::from_float<R>(z);
     if (QUANT)
-      a.q[at + c] = int8_t(__float2int_rn(__fmul_rn(y, s.inverse)));
+      a.q[at + c] = row::quantise(y, inverse);
     else
       static_cast<X*>(a.y)[at + c] = row::from_float<X>(y);
   }
 }
 
 template <typename X, typename R, bool QUANT>
-static cudaError_t launch(const Args& a, cudaStream_t stream) {
-  const row::RowPlan p = row::plan_row(a.N, a.C);
+static bool launch(const Args& a, cudaStream_t stream) {
   auto aligned = [](const void* ptr, size_t n) { return (reinterpret_cast<uintptr_t>(ptr) & (n - 1)) == 0; };
-  ++launch_counter();
-  if (p.units == 0) {
-    long_row_kernel<X, R, QUANT><<<unsigned(a.N), LONG_THREADS, 0, stream>>>(a);
-    return cudaPeekAtLastError();
-  }
-  // rows of 16-bit values that are a multiple of eight long all start at 16-byte boundaries
+  // rows that are a multiple of eight values long all start at 16-byte boundaries
   const bool vector = a.C % 8 == 0 && aligned(a.x, 16) && aligned(a.residual, 16) && aligned(a.weight, 16) &&
                       aligned(a.post_weight, 16) && (aligned(a.gate, 16) || !a.gate_per_channel) &&
                       aligned(a.z, 16) && (QUANT ? aligned(a.q, 8) : aligned(a.y, 16));
-  const dim3 block(p.threads(), p.rows_per_block());
-  const unsigned grid = unsigned((a.N + p.rows_per_block() - 1) / p.rows_per_block());
-  if (vector) {
-    if (p.units == 1) row_kernel<X, R, QUANT, true, 1><<<grid, block, 0, stream>>>(a);
-    else if (p.units == 2) row_kernel<X, R, QUANT, true, 2><<<grid, block, 0, stream>>>(a);
-    else row_kernel<X, R, QUANT, true, 4><<<grid, block, 0, stream>>>(a);
-  } else {
-    if (p.units == 1) row_kernel<X, R, QUANT, false, 1><<<grid, block, 0, stream>>>(a);
-    else if (p.units == 2) row_kernel<X, R, QUANT, false, 2><<<grid, block, 0, stream>>>(a);
-    else row_kernel<X, R, QUANT, false, 4><<<grid, block, 0, stream>>>(a);
-  }
-  return cudaPeekAtLastError();
+  // One group per thread is the shortest way through a row, for when rows do not fill the GPU;
+  // two measured best once they do (4096 x 8192 BF16, both norms, gate, quantised: 92 / 59 / 71 us
+  // for one / two / four).
+  const row::RowPlan r = row::plan_row(a.C, a.N < 512 && a.C <= 8192 ? 1 : 2, 1024, 1);
+  if (r.units == 0) return launch_on_stream(long_row_kernel<X, R, QUANT>, unsigned(a.N), LONG_THREADS, 0, 1, stream, a);
+  const dim3 block(r.threads, r.rows_per_block);
+  const unsigned grid = unsigned((a.N + r.rows_per_block - 1) / r.rows_per_block);
+  auto rows = [&](auto* kernel) { return launch_on_stream(kernel, grid, block, 0, 1, stream, a); };
+  if (vector)
+    return r.units == 1 ? rows(row_kernel<X, R, QUANT, row::VECTOR, 1>) : rows(row_kernel<X, R, QUANT, row::VECTOR, 2>);
+  return r.units == 1 ? rows(row_kernel<X, R, QUANT, row::STRIDED, 1>) : rows(row_kernel<X, R, QUANT, row::STRIDED, 2>);
 }
 
 template <bool QUANT>
 static int solve(const Args& a, int x_type, int residual_type, cudaStream_t stream) {
-  if (a.N <= 0 || a.N > 0x7fffffffLL || a.C <= 0 || !a.x || !a.residual || !a.weight || !a.z ||
+  if (a.N <= 0 || a.C <= 0 || !a.x || !a.residual || !a.weight || !a.z ||
       (QUANT ? !a.q || !a.scale : !a.y) || (a.gate && a.rows_per_gate <= 0) ||
       (residual_type != x_type && residual_type != row::TYPE_F32))
     return -1;
-  cudaError_t err;
+  if (x_type != row::TYPE_F16 && x_type != row::TYPE_BF16 && x_type != row::TYPE_F32) return -1;
+  const bool f32 = residual_type == row::TYPE_F32;
+  bool ok;
   if (x_type == row::TYPE_F16)
-    err = residual_type == row::TYPE_F32 ? launch<__half, float, QUANT>(a, stream)
-                                         : launch<__half, __half, QUANT>(a, stream);
+    ok = f32 ? launch<__half, float, QUANT>(a, stream) : launch<__half, __half, QUANT>(a, stream);
   else if (x_type == row::TYPE_BF16)
-    err = residual_type == row::TYPE_F32 ? launch<__nv_bfloat16, float, QUANT>(a, stream)
-                                         : launch<__nv_bfloat16, __nv_bfloat16, QUANT>(a, stream);
-  else if (x_type == row::TYPE_F32)
-    err = launch<float, float, QUANT>(a, stream);
+    ok = f32 ? launch<__nv_bfloat16, float, QUANT>(a, stream)
+             : launch<__nv_bfloat16, __nv_bfloat16, QUANT>(a, stream);
   else
-    return -1;
-  if (err != cudaSuccess) {
-    cudaGetLastError();
-    return -3;
-  }
-  return 0;
+    ok = launch<float, float, QUANT>(a, stream);
+  return ok ? 0 : -3;
 }
 
 }  // namespace bn
@@ -261,7 +259,7 @@ extern "C" int texo_block_norm_solve(const void* x, const void* residual, const 
                                      int x_type, int residual_type, int weights_f32, void* stream) {
   if (gate && (gate_rows <= 0 || N % gate_rows != 0)) return -1;
   texo::bn::Args a = {x, residual, weight, post_weight, gate, y, z, nullptr, nullptr, N, C,
-                      gate ? N / gate_rows : 1, gate_per_channel, eps, residual_scale, weights_f32};
+                      gate ? N / gate_rows : 1, gate_per_channel, eps, residual_scale, 1.f / float(C), weights_f32};
   return texo::bn::solve<false>(a, x_type, residual_type, static_cast<cudaStream_t>(stream));
 }
 
@@ -272,6 +270,6 @@ extern "C" int texo_block_norm_quant_solve(const void* x, const void* residual, 
                                            void* stream) {
   if (gate && (gate_rows <= 0 || N % gate_rows != 0)) return -1;
   texo::bn::Args a = {x, residual, weight, post_weight, gate, nullptr, z, q, scale, N, C,
-                      gate ? N / gate_rows : 1, gate_per_channel, eps, residual_scale, weights_f32};
+                      gate ? N / gate_rows : 1, gate_per_channel, eps, residual_scale, 1.f / float(C), weights_f32};
   return texo::bn::solve<true>(a, x_type, residual_type, static_cast<cudaStream_t>(stream));
 }

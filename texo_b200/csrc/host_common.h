@@ -186,6 +186,33 @@ inline long long& launch_counter() {
   return count;
 }
 
+// launch_overlapping_predecessor on the caller's stream, with a cluster size (1: none), counted;
+// false if the launch was refused.
+template <typename... Params, typename... Args>
+inline bool launch_on_stream(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem_bytes, int cluster,
+                             cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem_bytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attrs[2];
+  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  attrs[1].id = cudaLaunchAttributeClusterDimension;
+  attrs[1].val.clusterDim.x = unsigned(cluster);
+  attrs[1].val.clusterDim.y = 1;
+  attrs[1].val.clusterDim.z = 1;
+  cfg.attrs = attrs;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, Params(args)...) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  ++launch_counter();
+  return true;
+}
+
 // Optional CUDA-event bracket around the dominant kernel of each call, for roofline
 // reporting: while enabled, up to PROFILE_SLOTS launches are bracketed on the launching
 // stream; reading sums the elapsed times (and synchronises).

@@ -199,36 +199,6 @@ struct StreamBarriers {
 };
 static_assert(sizeof(StreamBarriers) <= 256, "StreamBarriers outgrew its shared-memory reserve");
 
-// Shared-memory accesses by address: the aligned base of the ring is computed from integers, so
-// the compiler would take accesses through its pointer for generic ones (measured 4 times as
-// slow in the shifting warps).
-__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ unsigned short lds16(uint32_t addr) {
-  unsigned short v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ int4 lds128(uint32_t addr) {
-  int4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(addr)
-               : "memory");
-  return v;
-}
-__device__ __forceinline__ void sts32(uint32_t addr, uint32_t v) {
-  asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
-}
-__device__ __forceinline__ void sts64(uint32_t addr, uint32_t x, uint32_t y) {
-  asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(addr), "r"(x), "r"(y) : "memory");
-}
-__device__ __forceinline__ void sts128(uint32_t addr, float x, float y, float z, float w) {
-  asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(x), "f"(y), "f"(z), "f"(w) : "memory");
-}
 __device__ __forceinline__ void store_cluster_u32(uint32_t cluster_addr, uint32_t v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
 }
@@ -1090,30 +1060,6 @@ static bool launch_generic(const int8_t* A, const int8_t* B, Y* out, int M, int 
   return cudaPeekAtLastError() == cudaSuccess;
 }
 
-// Launch in clusters of `cluster` CTAs; the grid may be scheduled while the one ahead drains.
-template <typename... Params, typename... Args>
-static bool launch_clusters(void (*kernel)(Params...), int grid, int threads, int smem_bytes, int cluster,
-                            cudaStream_t stream, Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem_bytes;
-  cfg.stream = stream;
-  cudaLaunchAttribute attrs[2];
-  attrs[0].id = cudaLaunchAttributeClusterDimension;
-  attrs[0].val.clusterDim.x = cluster;
-  attrs[0].val.clusterDim.y = 1;
-  attrs[0].val.clusterDim.z = 1;
-  attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attrs[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attrs;
-  cfg.numAttrs = 2;
-  ++launch_counter();
-  if (cudaLaunchKernelEx(&cfg, kernel, Params(args)...) == cudaSuccess) return true;
-  cudaGetLastError();
-  return false;
-}
-
 // Clusters of `cluster` CTAs that the device holds at once.
 template <typename Kernel>
 static int max_clusters(Kernel kernel, int threads, int smem_bytes, int cluster) {
@@ -1254,7 +1200,7 @@ static bool launch_stream(DeviceCtx& ctx, const StreamPlan& plan, const Operand&
     return false;
   const StreamShape p = {M, N, K, plan.R, plan.cluster, plan.m_tiles, plan.tiles,
                          N % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0};
-  return launch_clusters(stream_kernel<Y, GATHER>, plan.clusters * plan.cluster,
+  return launch_on_stream(stream_kernel<Y, GATHER>, plan.clusters * plan.cluster,
                          GATHER ? S_GATHER_THREADS : S_THREADS, s_smem_bytes(plan.R, GATHER), plan.cluster, stream,
                          map_b, map_a, A.p, B.p, out, s, p, ctx.status);
 }
@@ -1277,9 +1223,9 @@ static bool launch_pair(DeviceCtx& ctx, const DeviceSetup& d, const Operand& A, 
     return false;
   const PairShape p = {M, N, K, (M + 255) / 256, (N + 255) / 256, i8::raster_group_rows(K)};
   const int clusters = std::min(p.tiles_m * p.tiles_n, d.pairs);
-  return tma_out ? launch_clusters(pair_kernel<Y, true>, 2 * clusters, P_THREADS, P_SMEM_BYTES, 2, stream, map_a,
+  return tma_out ? launch_on_stream(pair_kernel<Y, true>, 2 * clusters, P_THREADS, P_SMEM_BYTES, 2, stream, map_a,
                                    map_b, map_y, out, s, p, ctx.status)
-                 : launch_clusters(pair_kernel<Y, false>, 2 * clusters, P_THREADS, P_SMEM_BYTES, 2, stream, map_a,
+                 : launch_on_stream(pair_kernel<Y, false>, 2 * clusters, P_THREADS, P_SMEM_BYTES, 2, stream, map_a,
                                    map_b, map_y, out, s, p, ctx.status);
 }
 
@@ -1299,7 +1245,7 @@ static bool launch_pad(const DeviceCtx& ctx, const Route& route, Operand& A, Ope
   }
   const long long a_pieces = a.pieces(), pieces = a_pieces + b.pieces();
   const int grid = int(std::min<long long>((pieces + PAD_THREADS / 32 - 1) / (PAD_THREADS / 32), ctx.sm_count * 8));
-  return launch_clusters(pad_kernel, grid, PAD_THREADS, 0, 1, stream, a, b, a_pieces, pieces);
+  return launch_on_stream(pad_kernel, grid, PAD_THREADS, 0, 1, stream, a, b, a_pieces, pieces);
 }
 
 static bool tma_can_move(const int8_t* p, int width) {

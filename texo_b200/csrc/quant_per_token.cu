@@ -7,7 +7,8 @@
 //   scale = max(amax|y|, 2^-100) / 127,  q = rint(y / scale)
 //
 // One scale per row needs the row's maximum before its first output, so the row stays in
-// registers between the two (row_ops.cuh): bound by HBM bandwidth, each byte crosses once.
+// registers between the two: bound by HBM bandwidth, each byte crosses once (row_ops.cuh).
+// Long rows are shared by a cluster of blocks that exchange their maxima.
 #include <cstdint>
 #include <cuda_runtime.h>
 
@@ -30,68 +31,90 @@ struct Args {
 };
 
 // gate and up are never multiplied first: their product can overflow where the result does not.
-// __expf and __fdividef are within a few units in the last place; a denominator beyond 2^126
-// (gate < -87) gives 0 where the value is below 2^-118.
+// The exponential is that of __expf (a product with log2 e, then ex2.approx), the reciprocal
+// rcp.approx; both flush subnormals, which saves the scaling around them: a denominator beyond
+// 2^126 (gate < -87) gives 0 where the value is below 2^-118.
 __device__ __forceinline__ float swiglu(float gate, float up) {
-  return __fdividef(gate, 1.f + __expf(-gate)) * up;
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmul_rn(gate, -1.44269504f)));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__fadd_rn(1.f, e)));
+  return gate * r * up;
 }
 
-// Group i of the row, as y.
-template <typename X, int FORM, bool VECTOR>
-__device__ __forceinline__ void load_y(const X* x, int C, int t, int threads, int i, float (&y)[8]) {
+// Group i of a row in global memory, as y; values past the end are zero.
+template <typename X, int FORM, row::Layout L>
+__device__ __forceinline__ void load_y(const X* x, const row::Spread<L>& s, int i, float (&y)[8]) {
   if (FORM == PLAIN) {
-    const row::Raw8<X> r = row::load_group<VECTOR>(x, C, t, threads, i);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = row::to_float(r.v[j]);
+    s.template load<true>(x, i, y);
   } else if (FORM == SWIGLU_HALVES) {
-    const row::Raw8<X> g = row::load_group<VECTOR>(x, C, t, threads, i);
-    const row::Raw8<X> u = row::load_group<VECTOR>(x + C, C, t, threads, i);
+    float g[8], u[8];
+    s.template load<true>(x, i, g);
+    s.template load<true>(x + s.C, i, u);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = swiglu(row::to_float(g.v[j]), row::to_float(u.v[j]));
-  } else if (VECTOR) {
-    const int c = row::position<true>(t, threads, i, 0);
-    if (c < C) {
-      const row::Raw8<X> lo = row::load8(x + 2 * c), hi = row::load8(x + 2 * c + 8);
+    for (int j = 0; j < 8; ++j) y[j] = swiglu(g[j], u[j]);
+  } else if (L == row::VECTOR) {
+    // the sixteen inputs of eight outputs: two groups of a row of 2 C values
+    const row::Spread<L> wide = {0, 1, 2 * s.C};
+    float lo[8], hi[8];
+    const int c = s.at(i, 0);
+    wide.template load<true>(x, c / 4, lo);
+    wide.template load<true>(x, c / 4 + 1, hi);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        y[j] = swiglu(row::to_float(lo.v[2 * j]), row::to_float(lo.v[2 * j + 1]));
-        y[4 + j] = swiglu(row::to_float(hi.v[2 * j]), row::to_float(hi.v[2 * j + 1]));
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = 0.f;
+    for (int j = 0; j < 4; ++j) {
+      y[j] = swiglu(lo[2 * j], lo[2 * j + 1]);
+      y[4 + j] = swiglu(hi[2 * j], hi[2 * j + 1]);
     }
-  } else {
+  } else if (sizeof(X) == 2 && (reinterpret_cast<uintptr_t>(x) & 3) == 0) {  // a pair is a word
+    unsigned w[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int c = row::position<false>(t, threads, i, j);
-      y[j] = c < C ? swiglu(row::to_float(__ldcs(x + 2 * size_t(c))), row::to_float(__ldcs(x + 2 * size_t(c) + 1)))
-                   : 0.f;
+      const int c = s.at(i, j);
+      w[j] = c < s.C ? __ldcs(reinterpret_cast<const unsigned int*>(x) + c) : 0u;
     }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float2 p = row::unpack2<X>(w[j]);
+      y[j] = swiglu(p.x, p.y);
+    }
+  } else {
+    X g[8], u[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int c = s.at(i, j);
+      g[j] = c < s.C ? __ldcs(x + 2 * size_t(c)) : row::from_float<X>(0.f);
+      u[j] = c < s.C ? __ldcs(x + 2 * size_t(c) + 1) : row::from_float<X>(0.f);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = swiglu(row::to_float(g[j]), row::to_float(u[j]));
   }
 }
 
-template <typename X, int FORM, bool VECTOR, int UNITS>
-__global__ void __launch_bounds__(UNITS == 4 ? 512 : 1024) row_kernel(const Args a) {
-  __shared__ unsigned scratch[row::MAX_WARPS];
-  const long long n = (long long)blockIdx.x * blockDim.y + threadIdx.y;
+// A block, a warp or (blocks > 1) a cluster per row.  blockDim = (threads, rows of the block).
+template <typename X, int FORM, row::Layout L, int UNITS>
+__global__ void __launch_bounds__(UNITS == 4 ? 512 : 1024) row_kernel(const Args a, int blocks) {
+  __shared__ unsigned scratch[row::MAX_WARPS], maxima[row::MAX_CLUSTER];
+  grid_dependency_trigger();
+  row::cluster_started(blocks);
+  const int part = int(blockIdx.x) % blocks;  // of the row
+  const long long n = (long long)(blockIdx.x / blocks) * blockDim.y + threadIdx.y;
   if (n >= a.N) return;  // only blocks of one-warp rows reach past N; they meet at no barrier
   const int t = threadIdx.x, threads = blockDim.x;
-  const X* x = static_cast<const X*>(a.x) + n * a.stride;
+  const row::Spread<L> s = {part * threads + t, blocks * threads, a.C};
+  grid_dependency_wait();
   float y[UNITS][8];
-  unsigned amax = 0;
 #pragma unroll
-  for (int i = 0; i < UNITS; ++i) load_y<X, FORM, VECTOR>(x, a.C, t, threads, i, y[i]);
+  for (int i = 0; i < UNITS; ++i) load_y<X, FORM>(static_cast<const X*>(a.x) + n * a.stride, s, i, y[i]);
+  float amax = 0.f;
 #pragma unroll
   for (int i = 0; i < UNITS; ++i) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(fabsf(y[i][j])));
+    for (int j = 0; j < 8; ++j) amax = row::max_abs(amax, y[i][j]);
   }
-  const row::TokenScale s = row::token_scale(row::row_max(amax, scratch, threads / 32));
-  if (t == 0) a.scale[n] = s.scale;
-  int8_t* q = a.q + size_t(n) * a.C;
+  amax = row::cluster_max(amax, scratch, t, threads / 32, maxima, blocks);
+  if (s.t == 0) a.scale[n] = row::token_scale(amax);
+  const float inverse = row::token_inverse(amax);
 #pragma unroll
-  for (int i = 0; i < UNITS; ++i) row::store_quantised<VECTOR>(q, a.C, t, threads, i, y[i], s.inverse);
+  for (int i = 0; i < UNITS; ++i) s.store_quantised(a.q + size_t(n) * a.C, i, y[i], inverse);
 }
 
 // Rows that the registers do not hold: y is computed twice.
@@ -99,6 +122,8 @@ constexpr int LONG_THREADS = 1024;
 template <typename X, int FORM>
 __global__ void __launch_bounds__(LONG_THREADS) long_row_kernel(const Args a) {
   __shared__ unsigned scratch[row::MAX_WARPS];
+  grid_dependency_trigger();
+  grid_dependency_wait();
   const long long n = blockIdx.x;
   const X* x = static_cast<const X*>(a.x) + n * a.stride;
   auto y_at = [&](int c) {
@@ -107,52 +132,49 @@ __global__ void __launch_bounds__(LONG_THREADS) long_row_kernel(const Args a) {
     const size_t u = FORM == SWIGLU_INTERLEAVED ? 2 * size_t(c) + 1 : size_t(a.C) + c;
     return swiglu(row::to_float(x[g]), row::to_float(x[u]));
   };
-  unsigned amax = 0;
-  for (int c = threadIdx.x; c < a.C; c += LONG_THREADS) amax = max(amax, __float_as_uint(fabsf(y_at(c))));
-  const row::TokenScale s = row::token_scale(row::row_max(amax, scratch, LONG_THREADS / 32));
-  if (threadIdx.x == 0) a.scale[n] = s.scale;
+  float amax = 0.f;
+  for (int c = threadIdx.x; c < a.C; c += LONG_THREADS) amax = row::max_abs(amax, y_at(c));
+  amax = row::row_max(amax, scratch, threadIdx.x, LONG_THREADS / 32);
+  if (threadIdx.x == 0) a.scale[n] = row::token_scale(amax);
+  const float inverse = row::token_inverse(amax);
   int8_t* q = a.q + size_t(n) * a.C;
-  for (int c = threadIdx.x; c < a.C; c += LONG_THREADS) q[c] = int8_t(__float2int_rn(__fmul_rn(y_at(c), s.inverse)));
+  for (int c = threadIdx.x; c < a.C; c += LONG_THREADS) q[c] = row::quantise(y_at(c), inverse);
 }
 
 template <typename X, int FORM>
-static cudaError_t launch(const Args& a, cudaStream_t stream) {
-  const row::RowPlan p = row::plan_row(a.N, a.C);
-  ++launch_counter();
-  if (p.units == 0) {
-    long_row_kernel<X, FORM><<<unsigned(a.N), LONG_THREADS, 0, stream>>>(a);
-    return cudaPeekAtLastError();
-  }
+static bool launch(const Args& a, cudaStream_t stream) {
   const bool vector = a.C % 8 == 0 && a.stride * sizeof(X) % 16 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 &&
                       (reinterpret_cast<uintptr_t>(a.q) & 7) == 0;
-  const dim3 block(p.threads(), p.rows_per_block());
-  const unsigned grid = unsigned((a.N + p.rows_per_block() - 1) / p.rows_per_block());
-  if (vector) {
-    if (p.units == 1) row_kernel<X, FORM, true, 1><<<grid, block, 0, stream>>>(a);
-    else if (p.units == 2) row_kernel<X, FORM, true, 2><<<grid, block, 0, stream>>>(a);
-    else row_kernel<X, FORM, true, 4><<<grid, block, 0, stream>>>(a);
-  } else {
-    if (p.units == 1) row_kernel<X, FORM, false, 1><<<grid, block, 0, stream>>>(a);
-    else if (p.units == 2) row_kernel<X, FORM, false, 2><<<grid, block, 0, stream>>>(a);
-    else row_kernel<X, FORM, false, 4><<<grid, block, 0, stream>>>(a);
-  }
-  return cudaPeekAtLastError();
+  // One group per thread while rows do not fill the GPU.  Once they do: four (8192 x 8192 BF16:
+  // 60 / 41 / 35 us for one / two / four), or two where 16-bit pairs are interleaved, whose groups
+  // are twice as wide (4096 x 11008: 45 / 50 us for two / four).
+  const bool wide = FORM == SWIGLU_INTERLEAVED && sizeof(X) == 2;
+  const row::RowPlan r = a.N < 512 ? row::plan_row(a.C, 1, 1024, row::MAX_CLUSTER)
+                         : wide    ? row::plan_row(a.C, 2, 768, row::MAX_CLUSTER)
+                                   : row::plan_row(a.C, 4, 512, row::MAX_CLUSTER);
+  if (r.units == 0 || a.N > 0x7fffffff / r.cluster)
+    return launch_on_stream(long_row_kernel<X, FORM>, unsigned(a.N), LONG_THREADS, 0, 1, stream, a);
+  const dim3 block(r.threads, r.rows_per_block);
+  const unsigned grid = unsigned((a.N + r.rows_per_block - 1) / r.rows_per_block) * r.cluster;
+  auto rows = [&](auto* kernel) { return launch_on_stream(kernel, grid, block, 0, r.cluster, stream, a, r.cluster); };
+  if (vector)
+    return r.units == 1   ? rows(row_kernel<X, FORM, row::VECTOR, 1>)
+           : r.units == 2 ? rows(row_kernel<X, FORM, row::VECTOR, 2>)
+                          : rows(row_kernel<X, FORM, row::VECTOR, 4>);
+  return r.units == 1   ? rows(row_kernel<X, FORM, row::STRIDED, 1>)
+         : r.units == 2 ? rows(row_kernel<X, FORM, row::STRIDED, 2>)
+                        : rows(row_kernel<X, FORM, row::STRIDED, 4>);
 }
 
 template <int FORM>
 static int solve(const Args& a, int x_type, cudaStream_t stream) {
   const long long width = FORM == PLAIN ? a.C : 2LL * a.C;
   if (a.N <= 0 || a.C <= 0 || a.stride < width || !a.x || !a.q || !a.scale) return -1;
-  cudaError_t err;
-  if (x_type == row::TYPE_F16) err = launch<__half, FORM>(a, stream);
-  else if (x_type == row::TYPE_BF16) err = launch<__nv_bfloat16, FORM>(a, stream);
-  else if (x_type == row::TYPE_F32) err = launch<float, FORM>(a, stream);
-  else return -1;
-  if (err != cudaSuccess) {
-    cudaGetLastError();
-    return -3;
-  }
-  return 0;
+  if (x_type != row::TYPE_F16 && x_type != row::TYPE_BF16 && x_type != row::TYPE_F32) return -1;
+  const bool ok = x_type == row::TYPE_F16    ? launch<__half, FORM>(a, stream)
+                  : x_type == row::TYPE_BF16 ? launch<__nv_bfloat16, FORM>(a, stream)
+                                             : launch<float, FORM>(a, stream);
+  return ok ? 0 : -3;
 }
 
 }  // namespace qt

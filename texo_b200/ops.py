@@ -451,10 +451,12 @@ class Int8Weights:
 
 
 # ---- dynamic quantisation: one activation scale per token.  These run on the caller's current
-# torch stream (the C entry points take it as an argument), use no scratch memory and may be
-# captured into a CUDA graph once the same call has been made outside of capture.
+# torch stream (the C entry points take it as an argument), own no scratch memory and may be
+# captured into a CUDA graph once the same call has been made outside of capture.  Their smallest
+# calls are bound by the host, so the checks are written to be cheap.
 
 _TYPE_CODES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_ENTRY_POINTS = {}
 
 
 def _check_float(name: str, t: torch.Tensor) -> int:
@@ -469,29 +471,35 @@ def _check_float(name: str, t: torch.Tensor) -> int:
     return code
 
 
-def _check_out(name: str, t: torch.Tensor | None, shape: tuple, dtype: torch.dtype,
-               like: torch.Tensor) -> torch.Tensor:
-    """The output tensor: a new one, or the caller's after its checks."""
-    if t is None:
-        return torch.empty(shape, dtype=dtype, device=like.device)
+def _check_out(name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype) -> torch.Tensor:
     _check_cuda(name, t, dtype)
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} has the wrong shape")
     return t
 
 
+def _matrix(like: torch.Tensor, rows: int, columns: int, dtype: torch.dtype) -> torch.Tensor:
+    return torch.empty_strided((rows, columns), (columns, 1), dtype=dtype, device=like.device)
+
+
+def _vector(like: torch.Tensor, n: int, dtype: torch.dtype) -> torch.Tensor:
+    return torch.empty_strided((n,), (1,), dtype=dtype, device=like.device)
+
+
 def _call_on_stream(name: str, like: torch.Tensor, others: tuple, *args) -> None:
     """Calls a stream-taking entry point on `like`'s device and that device's current stream."""
-    device = like.device
+    index = like.get_device()
     for t in others:
-        if t is not None and t.device != device:
+        if t is not None and t.get_device() != index:
             raise ValueError("all tensors must be on the same device")
-    fn = getattr(_lib.load(), name)
-    stream = torch._C._cuda_getCurrentRawStream(device.index)
-    if torch.cuda.current_device() == device.index:
+    fn = _ENTRY_POINTS.get(name)
+    if fn is None:
+        fn = _ENTRY_POINTS[name] = getattr(_lib.load(), name)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
         rc = fn(*args, stream)
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(index):
             rc = fn(*args, stream)
     if rc == -4:
         raise RuntimeError(f"{name}: make one call on this device before capturing a graph")
@@ -508,7 +516,8 @@ def mm_int8_per_token(A: torch.Tensor, B: torch.Tensor, scale_A: torch.Tensor, s
                       out: torch.Tensor | None = None) -> torch.Tensor:
     """Y[M,N] = float(sum_k A[m,k] B[k,n]) * scale_A[m] * scale_B[n] (+ bias[n]), rounded once to
     out_dtype (float16, bfloat16 or float32).  A [M,K], B [K,N] int8; scale_A [M], scale_B [N],
-    bias [N] float32, as quant_per_token and its relatives write them.  The dot is exact."""
+    bias [N] float32, as quant_per_token and its relatives write them.  The dot is exact.  Operands
+    that TMA cannot move (K or N not a multiple of 16) may be copied into a temporary tensor."""
     _check_cuda("A", A, torch.int8)
     _check_cuda("B", B, torch.int8)
     _check_cuda("scale_A", scale_A, torch.float32)
@@ -526,15 +535,15 @@ def mm_int8_per_token(A: torch.Tensor, B: torch.Tensor, scale_A: torch.Tensor, s
     code = _TYPE_CODES.get(out_dtype)
     if code is None:
         raise ValueError(f"out_dtype must be float16, bfloat16 or float32, got {out_dtype}")
-    out = _check_out("out", out, (M, N), out_dtype, A)
+    out = _matrix(A, M, N, out_dtype) if out is None else _check_out("out", out, (M, N), out_dtype)
     if M > 0:
         a, b = (A.data_ptr(), B.data_ptr()) if K else (None, None)
         workspace, size = None, 0
-        if K % 16 or N % 16 or (K and (a | b) % 16):  # operands that TMA cannot move may be copied
+        if K and (K % 16 or N % 16 or (a | b) % 16):  # operands that TMA cannot move
             with torch.cuda.device(A.device):
                 size = _lib.load().texo_mm_int8_per_token_workspace(a, b, M, N, K)
             if size:
-                workspace = torch.empty(size, dtype=torch.uint8, device=A.device)
+                workspace = _vector(A, size, torch.uint8)
         _call_on_stream("texo_mm_int8_solve_per_token", A, (B, scale_A, scale_B, bias, out), a, b, out.data_ptr(),
                         M, N, K, scale_A.data_ptr(), scale_B.data_ptr(), _ptr(bias), code, _ptr(workspace), size)
     return out
@@ -544,12 +553,13 @@ def _block_norm(quant, x, residual, weight, eps, post_weight, gate, residual_sca
     x_code = _check_float("x", x)
     residual_code = _check_float("residual", residual)
     weight_code = _check_float("weight", weight)
-    if x.dim() != 2 or residual.shape != x.shape or x.shape[1] <= 0 or weight.shape != (x.shape[1],):
+    shape = x.shape
+    if len(shape) != 2 or residual.shape != shape or shape[1] <= 0 or weight.shape != (shape[1],):
         raise ValueError("x, residual must be [N, C] with C > 0 and weight [C]")
-    N, C = x.shape
-    if residual_code not in (x_code, 2):
+    N, C = shape
+    if residual_code != x_code and residual_code != 2:
         raise ValueError("residual must have x's type or float32")
-    if weight_code not in (x_code, 2):
+    if weight_code != x_code and weight_code != 2:
         raise ValueError("weight must have x's type or float32")
     if post_weight is not None:
         _check_cuda("post_weight", post_weight, weight.dtype)
@@ -566,17 +576,24 @@ def _block_norm(quant, x, residual, weight, eps, post_weight, gate, residual_sca
             gate_per_channel = int(ok and gate.shape[1] == C)
         if not ok:
             raise ValueError("gate must be [C], [R, C] or [R, 1] with R dividing N")
-    out = _check_out("out", out, (N, C), torch.int8 if quant else x.dtype, x)
-    z = _check_out("z_out", z_out, (N, C), residual.dtype, x)
-    scale = _check_out("scale_out", scale_out, (N,), torch.float32, x) if quant else None
+    out_dtype = torch.int8 if quant else x.dtype
+    out = _matrix(x, N, C, out_dtype) if out is None else _check_out("out", out, (N, C), out_dtype)
+    z = _matrix(x, N, C, residual.dtype) if z_out is None else _check_out("z_out", z_out, (N, C), residual.dtype)
+    if quant:
+        scale = (_vector(x, N, torch.float32) if scale_out is None
+                 else _check_out("scale_out", scale_out, (N,), torch.float32))
+        if N > 0:
+            _call_on_stream("texo_block_norm_quant_solve", x, (residual, weight, post_weight, gate, out, z, scale),
+                            x.data_ptr(), residual.data_ptr(), weight.data_ptr(), _ptr(post_weight), _ptr(gate),
+                            out.data_ptr(), scale.data_ptr(), z.data_ptr(), N, C, gate_rows, gate_per_channel, eps,
+                            residual_scale, x_code, residual_code, weight_code == 2)
+        return out, scale, z
     if N > 0:
-        name = "texo_block_norm_quant_solve" if quant else "texo_block_norm_solve"
-        outs = (out.data_ptr(), scale.data_ptr()) if quant else (out.data_ptr(),)
-        _call_on_stream(name, x, (residual, weight, post_weight, gate, out, z, scale), x.data_ptr(),
-                        residual.data_ptr(), weight.data_ptr(), _ptr(post_weight), _ptr(gate), *outs, z.data_ptr(),
-                        N, C, gate_rows, gate_per_channel, eps, residual_scale, x_code, residual_code,
-                        int(weight_code == 2))
-    return (out, scale, z) if quant else (out, z)
+        _call_on_stream("texo_block_norm_solve", x, (residual, weight, post_weight, gate, out, z), x.data_ptr(),
+                        residual.data_ptr(), weight.data_ptr(), _ptr(post_weight), _ptr(gate), out.data_ptr(),
+                        z.data_ptr(), N, C, gate_rows, gate_per_channel, eps, residual_scale, x_code, residual_code,
+                        weight_code == 2)
+    return out, z
 
 
 def block_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float,
@@ -611,11 +628,18 @@ def _check_rows(name: str, t: torch.Tensor) -> int:
     code = _TYPE_CODES.get(t.dtype)
     if code is None:
         raise ValueError(f"{name} must be float16, bfloat16 or float32, got {t.dtype}")
-    if t.dim() != 2 or t.shape[1] <= 0:
+    shape = t.shape
+    if len(shape) != 2 or shape[1] <= 0:
         raise ValueError(f"{name} must be a matrix with at least one column")
-    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+    if not t.is_contiguous() and ((shape[1] > 1 and t.stride(1) != 1) or (shape[0] > 1 and t.stride(0) < shape[1])):
         raise ValueError(f"{name} must be row-major with rows that do not overlap")
     return code
+
+
+def _quantised(x, N, C, out, scale_out):
+    return (_matrix(x, N, C, torch.int8) if out is None else _check_out("out", out, (N, C), torch.int8),
+            _vector(x, N, torch.float32) if scale_out is None
+            else _check_out("scale_out", scale_out, (N,), torch.float32))
 
 
 def quant_per_token(x: torch.Tensor, out: torch.Tensor | None = None,
@@ -625,8 +649,7 @@ def quant_per_token(x: torch.Tensor, out: torch.Tensor | None = None,
     that holds a NaN or an infinity gets scale NaN and q = 0."""
     code = _check_rows("x", x)
     N, C = x.shape
-    q = _check_out("out", out, (N, C), torch.int8, x)
-    scale = _check_out("scale_out", scale_out, (N,), torch.float32, x)
+    q, scale = _quantised(x, N, C, out, scale_out)
     if N > 0:
         _call_on_stream("texo_quant_per_token_solve", x, (q, scale), x.data_ptr(), q.data_ptr(), scale.data_ptr(),
                         N, C, max(x.stride(0), C), code)
@@ -639,14 +662,13 @@ def swiglu_quant_per_token(gate_up: torch.Tensor, interleaved: bool = True, out:
     j at 2j, up j at 2j + 1, the order of mm_int8_swiglu's weights) or side by side.  Returns (q
     int8 [N,F], scale float32 [N])."""
     code = _check_rows("gate_up", gate_up)
-    N, F = gate_up.shape[0], gate_up.shape[1] // 2
-    if gate_up.shape[1] % 2:
+    N, width = gate_up.shape
+    if width % 2:
         raise ValueError("gate_up must have an even number of columns")
-    q = _check_out("out", out, (N, F), torch.int8, gate_up)
-    scale = _check_out("scale_out", scale_out, (N,), torch.float32, gate_up)
+    q, scale = _quantised(gate_up, N, width // 2, out, scale_out)
     if N > 0:
         _call_on_stream("texo_swiglu_quant_per_token_solve", gate_up, (q, scale), gate_up.data_ptr(), q.data_ptr(),
-                        scale.data_ptr(), N, F, max(gate_up.stride(0), 2 * F), int(bool(interleaved)), code)
+                        scale.data_ptr(), N, width // 2, max(gate_up.stride(0), width), bool(interleaved), code)
     return q, scale
 
 
