@@ -147,9 +147,11 @@ static bool launch(const Args& a, cudaStream_t stream) {
                       (reinterpret_cast<uintptr_t>(a.q) & 7) == 0;
   // One group per thread while rows do not fill the GPU.  Once they do: four (8192 x 8192 BF16:
   // 60 / 41 / 35 us for one / two / four), or two where 16-bit pairs are interleaved, whose groups
-  // are twice as wide (4096 x 11008: 45 / 50 us for two / four).
+  // are twice as wide (4096 x 11008: 45 / 50 us for two / four), and in unaligned rows, whose
+  // addresses fill the registers (1023 x 11007 halves: 34 / 29 / 40 us).
   const bool wide = FORM == SWIGLU_INTERLEAVED && sizeof(X) == 2;
   const row::RowPlan r = a.N < 512 ? row::plan_row(a.C, 1, 1024, row::MAX_CLUSTER)
+                         : !vector ? row::plan_row(a.C, 2, 1024, row::MAX_CLUSTER)
                          : wide    ? row::plan_row(a.C, 2, 768, row::MAX_CLUSTER)
                                    : row::plan_row(a.C, 4, 512, row::MAX_CLUSTER);
   if (r.units == 0 || a.N > 0x7fffffff / r.cluster)
@@ -161,9 +163,7 @@ static bool launch(const Args& a, cudaStream_t stream) {
     return r.units == 1   ? rows(row_kernel<X, FORM, row::VECTOR, 1>)
            : r.units == 2 ? rows(row_kernel<X, FORM, row::VECTOR, 2>)
                           : rows(row_kernel<X, FORM, row::VECTOR, 4>);
-  return r.units == 1   ? rows(row_kernel<X, FORM, row::STRIDED, 1>)
-         : r.units == 2 ? rows(row_kernel<X, FORM, row::STRIDED, 2>)
-                        : rows(row_kernel<X, FORM, row::STRIDED, 4>);
+  return r.units == 1 ? rows(row_kernel<X, FORM, row::STRIDED, 1>) : rows(row_kernel<X, FORM, row::STRIDED, 2>);
 }
 
 template <int FORM>

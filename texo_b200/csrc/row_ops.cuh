@@ -150,8 +150,8 @@ struct Spread {
       T raw[8];  // all loads before the first conversion
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int c = at(i, j);
-        raw[j] = c < C ? (ONCE ? __ldcs(row + c) : row[c]) : from_float<T>(0.f);
+        const unsigned c = at(i, j);
+        raw[j] = c < unsigned(C) ? (ONCE ? __ldcs(row + c) : row[c]) : from_float<T>(0.f);
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = to_float(raw[j]);
@@ -165,7 +165,7 @@ struct Spread {
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (at(i, j) < C) __stcs(row + at(i, j), from_float<T>(v[j]));
+        if (at(i, j) < C) __stcs(row + unsigned(at(i, j)), from_float<T>(v[j]));
     }
   }
 
@@ -187,7 +187,7 @@ struct Spread {
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (at(i, j) < C) row[at(i, j)] = int8_t(uint8_t(r[j]));
+        if (at(i, j) < C) row[unsigned(at(i, j))] = int8_t(uint8_t(r[j]));
     }
   }
 };
