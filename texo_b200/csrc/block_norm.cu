@@ -79,23 +79,22 @@ __device__ __forceinline__ void to_u(const Args& a, size_t gate_row, const row::
   }
 }
 
-// u and the residual (group i) -> z, in registers and to memory.  Values past the row's end become
+// u and the residual (group i) -> z, in registers and to the row at `z`.  Values past the row's end become
 // zero whatever they were.
 template <typename R, row::Layout L>
-__device__ __forceinline__ void to_z(const Args& a, int n, const row::Spread<L>& s, int i, const float (&r)[8],
+__device__ __forceinline__ void to_z(const Args& a, R* z, const row::Spread<L>& s, int i, const float (&r)[8],
                                      float (&v)[8]) {
   row::fma8(v, r, a.residual_scale, v);
   s.mask(i, v);
-  s.store(static_cast<R*>(a.z) + size_t(n) * a.C, i, v);
+  s.store(z, i, v);
 }
 
-// z -> the outputs.
+// z -> the outputs, to the row at `y` or `q`.
 template <typename X, bool QUANT, row::Layout L, int UNITS>
-__device__ __forceinline__ void finish(const Args& a, int n, const row::Spread<L>& s, float (&v)[UNITS][8],
-                                       float* sum_scratch, unsigned* max_scratch) {
+__device__ __forceinline__ void finish(const Args& a, int n, X* y, int8_t* q, const row::Spread<L>& s,
+                                       float (&v)[UNITS][8], float* sum_scratch, unsigned* max_scratch) {
   const int warps = s.threads / 32;
   const float inv = rsqrtf(row::row_sum(squares(v), sum_scratch, s.t, warps) * a.inv_c + a.eps);
-  const size_t at = size_t(n) * a.C;
   float amax = 0.f;
 #pragma unroll
   for (int i = 0; i < UNITS; ++i) {
@@ -108,7 +107,7 @@ __device__ __forceinline__ void finish(const Args& a, int n, const row::Spread<L
 #pragma unroll
       for (int j = 0; j < 8; ++j) amax = row::max_abs(amax, v[i][j]);
     } else {
-      s.store(static_cast<X*>(a.y) + at, i, v[i]);
+      s.store(y, i, v[i]);
     }
   }
   if (QUANT) {
@@ -116,7 +115,7 @@ __device__ __forceinline__ void finish(const Args& a, int n, const row::Spread<L
     if (s.t == 0) a.scale[n] = row::token_scale(amax);
     const float inverse = row::token_inverse(amax);
 #pragma unroll
-    for (int i = 0; i < UNITS; ++i) s.store_quantised(a.q + at, i, v[i], inverse);
+    for (int i = 0; i < UNITS; ++i) s.store_quantised(q, i, v[i], inverse);
   }
 }
 
@@ -135,21 +134,59 @@ __global__ void __launch_bounds__(1024) row_kernel(const Args a) {
   const int n = int(row_number);
   const row::Spread<L> s = {int(threadIdx.x), int(blockDim.x), a.C};
   const size_t gate_row = a.gate ? size_t(unsigned(n) / unsigned(a.rows_per_gate)) : 0;
+  const size_t at = size_t(n) * a.C;
+  R* z = static_cast<R*>(a.z) + at;
+  X* y = static_cast<X*>(a.y) + at;
+  int8_t* q = a.q + at;
   grid_dependency_wait();
   float v[UNITS][8], r[UNITS][8];
+  if constexpr (L == row::ALIGNED) {
 #pragma unroll
-  for (int i = 0; i < UNITS; ++i) s.template load<true>(static_cast<const X*>(a.x) + size_t(n) * a.C, i, v[i]);
+    for (int i = 0; i < UNITS; ++i) s.template load<true>(static_cast<const X*>(a.x) + at, i, v[i]);
 #pragma unroll
-  for (int i = 0; i < UNITS; ++i) s.template load<true>(static_cast<const R*>(a.residual) + size_t(n) * a.C, i, r[i]);
+    for (int i = 0; i < UNITS; ++i) s.template load<true>(static_cast<const R*>(a.residual) + at, i, r[i]);
+  } else {
+    // x's room takes y or q afterwards, the residual's z
+    extern __shared__ __align__(16) uint8_t staging[];
+    uint8_t* staged_r = staging + row::staged_bytes((long long)a.C * sizeof(X));
+    auto fetch = [&](const void* base, int size, uint8_t* to) {
+      const uintptr_t begin = reinterpret_cast<uintptr_t>(base), src = begin + at * size;
+      row::fetch_row(smem_u32(to), src, a.C * size, begin, begin + size_t(a.N) * a.C * size, s.t, s.threads);
+      return unsigned(src & 15);
+    };
+    const unsigned x_offset = fetch(a.x, sizeof(X), staging), r_offset = fetch(a.residual, sizeof(R), staged_r);
+    row::fetched();
+#pragma unroll
+    for (int i = 0; i < UNITS; ++i) {
+      if (s.at(i, 0) < a.C) {
+        row::read_staged<X>(smem_u32(staging), x_offset, s.at(i, 0), v[i]);
+        row::read_staged<R>(smem_u32(staged_r), r_offset, s.at(i, 0), r[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = r[i][j] = 0.f;
+      }
+      s.mask(i, v[i]);  // (what lies past the row's end is arbitrary)
+    }
+    __syncthreads();
+    z = reinterpret_cast<R*>(staged_r);
+    y = reinterpret_cast<X*>(staging);
+    q = reinterpret_cast<int8_t*>(staging);
+  }
   float post_inv = 1.f;
   if (a.post_weight)
     post_inv = rsqrtf(row::row_sum(squares(v), scratch.post, s.t, s.threads / 32) * a.inv_c + a.eps);
 #pragma unroll
   for (int i = 0; i < UNITS; ++i) {
     to_u<X>(a, gate_row, s, i, post_inv, v[i]);
-    to_z<R>(a, n, s, i, r[i], v[i]);
+    to_z(a, z, s, i, r[i], v[i]);
   }
-  finish<X, QUANT>(a, n, s, v, scratch.sum, scratch.max);
+  finish<X, QUANT>(a, n, y, q, s, v, scratch.sum, scratch.max);
+  if constexpr (L == row::STAGED) {
+    __syncthreads();
+    row::send_row(reinterpret_cast<uintptr_t>(static_cast<R*>(a.z) + at), smem_u32(z), a.C * int(sizeof(R)), s.t, s.threads);
+    if (QUANT) row::send_row(reinterpret_cast<uintptr_t>(a.q + at), smem_u32(q), a.C, s.t, s.threads);
+    else row::send_row(reinterpret_cast<uintptr_t>(static_cast<X*>(a.y) + at), smem_u32(y), a.C * int(sizeof(X)), s.t, s.threads);
+  }
 }
 
 // Rows that the registers do not hold: the values are computed again from x and residual in
@@ -215,20 +252,23 @@ template <typename X, typename R, bool QUANT>
 static bool launch(const Args& a, cudaStream_t stream) {
   auto aligned = [](const void* ptr, size_t n) { return (reinterpret_cast<uintptr_t>(ptr) & (n - 1)) == 0; };
   // rows that are a multiple of eight values long all start at 16-byte boundaries
-  const bool vector = a.C % 8 == 0 && aligned(a.x, 16) && aligned(a.residual, 16) && aligned(a.weight, 16) &&
+  const bool aligned_rows = a.C % 8 == 0 && aligned(a.x, 16) && aligned(a.residual, 16) && aligned(a.weight, 16) &&
                       aligned(a.post_weight, 16) && (aligned(a.gate, 16) || !a.gate_per_channel) &&
                       aligned(a.z, 16) && (QUANT ? aligned(a.q, 8) : aligned(a.y, 16));
   // One group per thread is the shortest way through a row, for when rows do not fill the GPU;
   // two measured best once they do (4096 x 8192 BF16, both norms, gate, quantised: 92 / 59 / 71 us
   // for one / two / four).
-  const row::RowPlan r = row::plan_row(a.C, a.N < 512 && a.C <= 8192 ? 1 : 2, 1024, 1);
+  const row::RowPlan r = row::plan_row(a.C, a.N < 512 && a.C <= 8192 ? 1 : 2, 1024, 1, aligned_rows);
   if (r.units == 0) return launch_on_stream(long_row_kernel<X, R, QUANT>, unsigned(a.N), LONG_THREADS, 0, 1, stream, a);
   const dim3 block(r.threads, r.rows_per_block);
   const unsigned grid = unsigned((a.N + r.rows_per_block - 1) / r.rows_per_block);
-  auto rows = [&](auto* kernel) { return launch_on_stream(kernel, grid, block, 0, 1, stream, a); };
-  if (vector)
-    return r.units == 1 ? rows(row_kernel<X, R, QUANT, row::VECTOR, 1>) : rows(row_kernel<X, R, QUANT, row::VECTOR, 2>);
-  return r.units == 1 ? rows(row_kernel<X, R, QUANT, row::STRIDED, 1>) : rows(row_kernel<X, R, QUANT, row::STRIDED, 2>);
+  if (aligned_rows)
+    return r.units == 1
+               ? launch_on_stream(row_kernel<X, R, QUANT, row::ALIGNED, 1>, grid, block, 0, 1, stream, a)
+               : launch_on_stream(row_kernel<X, R, QUANT, row::ALIGNED, 2>, grid, block, 0, 1, stream, a);
+  const int room = row::staged_bytes((long long)a.C * sizeof(X)) + row::staged_bytes((long long)a.C * sizeof(R));
+  return r.units == 1 ? row::launch_staged(row_kernel<X, R, QUANT, row::STAGED, 1>, grid, block, room, stream, a)
+                      : row::launch_staged(row_kernel<X, R, QUANT, row::STAGED, 2>, grid, block, room, stream, a);
 }
 
 template <bool QUANT>

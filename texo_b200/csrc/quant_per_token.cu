@@ -41,9 +41,18 @@ __device__ __forceinline__ float swiglu(float gate, float up) {
   return gate * r * up;
 }
 
-// Group i of a row in global memory, as y; values past the end are zero.
-template <typename X, int FORM, row::Layout L>
-__device__ __forceinline__ void load_y(const X* x, const row::Spread<L>& s, int i, float (&y)[8]) {
+// Eight outputs from sixteen interleaved inputs.
+__device__ __forceinline__ void swiglu_pairs(const float (&lo)[8], const float (&hi)[8], float (&y)[8]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    y[j] = swiglu(lo[2 * j], lo[2 * j + 1]);
+    y[4 + j] = swiglu(hi[2 * j], hi[2 * j + 1]);
+  }
+}
+
+// Group i of an aligned row in global memory, as y; values past the end are zero.
+template <typename X, int FORM>
+__device__ __forceinline__ void load_y(const X* x, const row::Spread<row::ALIGNED>& s, int i, float (&y)[8]) {
   if (FORM == PLAIN) {
     s.template load<true>(x, i, y);
   } else if (FORM == SWIGLU_HALVES) {
@@ -52,46 +61,45 @@ __device__ __forceinline__ void load_y(const X* x, const row::Spread<L>& s, int 
     s.template load<true>(x + s.C, i, u);
 #pragma unroll
     for (int j = 0; j < 8; ++j) y[j] = swiglu(g[j], u[j]);
-  } else if (L == row::VECTOR) {
+  } else {
     // the sixteen inputs of eight outputs: two groups of a row of 2 C values
-    const row::Spread<L> wide = {0, 1, 2 * s.C};
+    const row::Spread<row::ALIGNED> wide = {0, 1, 2 * s.C};
     float lo[8], hi[8];
     const int c = s.at(i, 0);
     wide.template load<true>(x, c / 4, lo);
     wide.template load<true>(x, c / 4 + 1, hi);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      y[j] = swiglu(lo[2 * j], lo[2 * j + 1]);
-      y[4 + j] = swiglu(hi[2 * j], hi[2 * j + 1]);
-    }
-  } else if (sizeof(X) == 2 && (reinterpret_cast<uintptr_t>(x) & 3) == 0) {  // a pair is a word
-    unsigned w[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = s.at(i, j);
-      w[j] = c < s.C ? __ldcs(reinterpret_cast<const unsigned int*>(x) + c) : 0u;
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float2 p = row::unpack2<X>(w[j]);
-      y[j] = swiglu(p.x, p.y);
-    }
-  } else {
-    X g[8], u[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = s.at(i, j);
-      g[j] = c < s.C ? __ldcs(x + 2 * size_t(c)) : row::from_float<X>(0.f);
-      u[j] = c < s.C ? __ldcs(x + 2 * size_t(c) + 1) : row::from_float<X>(0.f);
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = swiglu(row::to_float(g[j]), row::to_float(u[j]));
+    swiglu_pairs(lo, hi, y);
   }
+}
+// The same of a staged row: `first` holds x (or the gates, `second` the ups).
+template <typename X, int FORM>
+__device__ __forceinline__ void read_y(uint32_t first, unsigned offset, uint32_t second, unsigned second_offset,
+                                       const row::Spread<row::STAGED>& s, int i, float (&y)[8]) {
+  if (s.at(i, 0) >= s.C) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = 0.f;
+    return;
+  }
+  if (FORM == SWIGLU_INTERLEAVED) {
+    float lo[8], hi[8];
+    row::read_staged<X>(first, offset, 2 * s.at(i, 0), lo);
+    row::read_staged<X>(first, offset, 2 * s.at(i, 0) + 8, hi);
+    swiglu_pairs(lo, hi, y);
+  } else {
+    row::read_staged<X>(first, offset, s.at(i, 0), y);
+    if (FORM == SWIGLU_HALVES) {
+      float u[8];
+      row::read_staged<X>(second, second_offset, s.at(i, 0), u);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = swiglu(y[j], u[j]);
+    }
+  }
+  s.mask(i, y);  // (what lies past the row's end is arbitrary)
 }
 
 // A block, a warp or (blocks > 1) a cluster per row.  blockDim = (threads, rows of the block).
 template <typename X, int FORM, row::Layout L, int UNITS>
-__global__ void __launch_bounds__(UNITS == 4 ? 512 : 1024) row_kernel(const Args a, int blocks) {
+__global__ void __launch_bounds__(UNITS == 4 && L == row::ALIGNED ? 512 : 1024) row_kernel(const Args a, int blocks) {
   __shared__ unsigned scratch[row::MAX_WARPS], maxima[row::MAX_CLUSTER];
   grid_dependency_trigger();
   row::cluster_started(blocks);
@@ -100,10 +108,29 @@ __global__ void __launch_bounds__(UNITS == 4 ? 512 : 1024) row_kernel(const Args
   if (n >= a.N) return;  // only blocks of one-warp rows reach past N; they meet at no barrier
   const int t = threadIdx.x, threads = blockDim.x;
   const row::Spread<L> s = {part * threads + t, blocks * threads, a.C};
+  const X* x = static_cast<const X*>(a.x) + n * a.stride;
+  int8_t* q = a.q + size_t(n) * a.C;
   grid_dependency_wait();
   float y[UNITS][8];
+  if constexpr (L == row::ALIGNED) {
 #pragma unroll
-  for (int i = 0; i < UNITS; ++i) load_y<X, FORM>(static_cast<const X*>(a.x) + n * a.stride, s, i, y[i]);
+    for (int i = 0; i < UNITS; ++i) load_y<X, FORM>(x, s, i, y[i]);
+  } else {  // a block per row; x's room takes q afterwards
+    extern __shared__ __align__(16) uint8_t staging[];
+    const uintptr_t begin = reinterpret_cast<uintptr_t>(a.x);
+    const uintptr_t end = begin + size_t((a.N - 1) * a.stride + (long long)a.C * (FORM == PLAIN ? 1 : 2)) * sizeof(X);
+    const int bytes = a.C * int(sizeof(X)) * (FORM == SWIGLU_INTERLEAVED ? 2 : 1);
+    const uintptr_t first = reinterpret_cast<uintptr_t>(x), second = reinterpret_cast<uintptr_t>(x + a.C);
+    const uint32_t to = smem_u32(staging), to_second = to + row::staged_bytes(bytes);
+    row::fetch_row(to, first, bytes, begin, end, t, threads);
+    if (FORM == SWIGLU_HALVES) row::fetch_row(to_second, second, bytes, begin, end, t, threads);
+    row::fetched();
+#pragma unroll
+    for (int i = 0; i < UNITS; ++i)
+      read_y<X, FORM>(to, unsigned(first & 15), to_second, unsigned(second & 15), s, i, y[i]);
+    __syncthreads();
+    q = reinterpret_cast<int8_t*>(staging);
+  }
   float amax = 0.f;
 #pragma unroll
   for (int i = 0; i < UNITS; ++i) {
@@ -114,7 +141,11 @@ __global__ void __launch_bounds__(UNITS == 4 ? 512 : 1024) row_kernel(const Args
   if (s.t == 0) a.scale[n] = row::token_scale(amax);
   const float inverse = row::token_inverse(amax);
 #pragma unroll
-  for (int i = 0; i < UNITS; ++i) s.store_quantised(a.q + size_t(n) * a.C, i, y[i], inverse);
+  for (int i = 0; i < UNITS; ++i) s.store_quantised(q, i, y[i], inverse);
+  if constexpr (L == row::STAGED) {
+    __syncthreads();
+    row::send_row(reinterpret_cast<uintptr_t>(a.q + size_t(n) * a.C), smem_u32(q), a.C, t, threads);
+  }
 }
 
 // Rows that the registers do not hold: y is computed twice.
@@ -143,27 +174,32 @@ __global__ void __launch_bounds__(LONG_THREADS) long_row_kernel(const Args a) {
 
 template <typename X, int FORM>
 static bool launch(const Args& a, cudaStream_t stream) {
-  const bool vector = a.C % 8 == 0 && a.stride * sizeof(X) % 16 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 &&
-                      (reinterpret_cast<uintptr_t>(a.q) & 7) == 0;
+  const bool aligned_rows = a.C % 8 == 0 && a.stride * sizeof(X) % 16 == 0 &&
+                            (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && (reinterpret_cast<uintptr_t>(a.q) & 7) == 0;
+  auto launch_long = [&] { return launch_on_stream(long_row_kernel<X, FORM>, unsigned(a.N), LONG_THREADS, 0, 1, stream, a); };
+  if (!aligned_rows) {
+    const int bytes = a.C <= 32768 ? a.C * int(sizeof(X)) * (FORM == SWIGLU_INTERLEAVED ? 2 : 1) : 0;
+    const int room = row::staged_bytes(bytes) * (FORM == SWIGLU_HALVES ? 2 : 1);
+    // (4000 x 11007 BF16: 85 / 51 us for two / four groups per thread)
+    const row::RowPlan r = row::plan_row(a.C, a.N < 512 && a.C <= 8192 ? 1 : 4, 1024, 1, false);
+    if (r.units == 0 || room > row::SMEM_LIMIT) return launch_long();
+    auto rows = [&](auto* kernel) { return row::launch_staged(kernel, unsigned(a.N), dim3(r.threads), room, stream, a, 1); };
+    return r.units == 1 ? rows(row_kernel<X, FORM, row::STAGED, 1>) : rows(row_kernel<X, FORM, row::STAGED, 4>);
+  }
   // One group per thread while rows do not fill the GPU.  Once they do: four (8192 x 8192 BF16:
   // 60 / 41 / 35 us for one / two / four), or two where 16-bit pairs are interleaved, whose groups
-  // are twice as wide (4096 x 11008: 45 / 50 us for two / four), and in unaligned rows, whose
-  // addresses fill the registers (1023 x 11007 halves: 34 / 29 / 40 us).
+  // are twice as wide (4096 x 11008: 45 / 50 us for two / four).
   const bool wide = FORM == SWIGLU_INTERLEAVED && sizeof(X) == 2;
-  const row::RowPlan r = a.N < 512 ? row::plan_row(a.C, 1, 1024, row::MAX_CLUSTER)
-                         : !vector ? row::plan_row(a.C, 2, 1024, row::MAX_CLUSTER)
-                         : wide    ? row::plan_row(a.C, 2, 768, row::MAX_CLUSTER)
-                                   : row::plan_row(a.C, 4, 512, row::MAX_CLUSTER);
-  if (r.units == 0 || a.N > 0x7fffffff / r.cluster)
-    return launch_on_stream(long_row_kernel<X, FORM>, unsigned(a.N), LONG_THREADS, 0, 1, stream, a);
+  const row::RowPlan r = a.N < 512 ? row::plan_row(a.C, 1, 1024, row::MAX_CLUSTER, true)
+                         : wide    ? row::plan_row(a.C, 2, 768, row::MAX_CLUSTER, true)
+                                   : row::plan_row(a.C, 4, 512, row::MAX_CLUSTER, true);
+  if (r.units == 0 || a.N > 0x7fffffff / r.cluster) return launch_long();
   const dim3 block(r.threads, r.rows_per_block);
   const unsigned grid = unsigned((a.N + r.rows_per_block - 1) / r.rows_per_block) * r.cluster;
   auto rows = [&](auto* kernel) { return launch_on_stream(kernel, grid, block, 0, r.cluster, stream, a, r.cluster); };
-  if (vector)
-    return r.units == 1   ? rows(row_kernel<X, FORM, row::VECTOR, 1>)
-           : r.units == 2 ? rows(row_kernel<X, FORM, row::VECTOR, 2>)
-                          : rows(row_kernel<X, FORM, row::VECTOR, 4>);
-  return r.units == 1 ? rows(row_kernel<X, FORM, row::STRIDED, 1>) : rows(row_kernel<X, FORM, row::STRIDED, 2>);
+  return r.units == 1   ? rows(row_kernel<X, FORM, row::ALIGNED, 1>)
+         : r.units == 2 ? rows(row_kernel<X, FORM, row::ALIGNED, 2>)
+                        : rows(row_kernel<X, FORM, row::ALIGNED, 4>);
 }
 
 template <int FORM>

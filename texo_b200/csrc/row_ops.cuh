@@ -16,6 +16,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include "host_common.h"
 #include "ptx.cuh"
 #include "requant.cuh"
 
@@ -109,19 +110,15 @@ __device__ __forceinline__ void mul8(float (&v)[8], const A& a, const B& b) {
   }
 }
 
-// A row of C values over `threads` threads, this one being thread t, in groups of eight values:
-//   VECTOR   group i is eight neighbouring values (rows start at 16-byte boundaries)
-//   STRIDED  single values, each next to that of the next thread (any alignment).  Words of two
-//            16-bit values, shifted into place in rows that start half way through one, halve the
-//            loads but cost more instructions than that saves: 70 us against 38 on 2050 x 4999 FP16.
-enum Layout { VECTOR, STRIDED };
+// A row of C values over `threads` threads, this one being thread t: group i is the eight values
+// from at(i, 0) on.
+//   ALIGNED  rows start at 16-byte boundaries and are a multiple of eight long
+//   STAGED   any rows: they pass through shared memory (see below)
+enum Layout { ALIGNED, STAGED };
 template <Layout L>
 struct Spread {
   int t, threads, C;
-  __device__ __forceinline__ int at(int i, int j) const {
-    if (L == VECTOR) return (i * threads + t) * 8 + j;
-    return t + (i * 8 + j) * threads;
-  }
+  __device__ __forceinline__ int at(int i, int j) const { return (i * threads + t) * 8 + j; }
 
   // Whether group i of every thread lies within the row.
   __device__ __forceinline__ bool full(int i) const { return (i + 1) * threads * 8 <= C; }
@@ -136,40 +133,39 @@ struct Spread {
   // Group i of a row in global memory; values past the end read as zero.  ONCE: not worth caching.
   template <bool ONCE, typename T>
   __device__ __forceinline__ void load(const T* row, int i, float (&v)[8]) const {
-    if (L == VECTOR) {
-      Raw8<T> r;
+    Raw8<T> r;
+    if (L == ALIGNED || ((reinterpret_cast<uintptr_t>(row) & 15) == 0 && at(i, 8) <= C)) {
       uint4* d = reinterpret_cast<uint4*>(&r);
       const uint4* s = reinterpret_cast<const uint4*>(row + at(i, 0));
       const bool in = at(i, 0) < C;
 #pragma unroll
       for (int k = 0; k < int(sizeof(Raw8<T>) / 16); ++k)
         d[k] = !in ? make_uint4(0, 0, 0, 0) : ONCE ? __ldcs(s + k) : __ldg(s + k);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = to_float(r.v[j]);
     } else {
-      T raw[8];  // all loads before the first conversion
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const unsigned c = at(i, j);
-        raw[j] = c < unsigned(C) ? (ONCE ? __ldcs(row + c) : row[c]) : from_float<T>(0.f);
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = to_float(raw[j]);
+      for (int j = 0; j < 8; ++j) r.v[j] = at(i, j) < C ? row[at(i, j)] : from_float<T>(0.f);
     }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = to_float(r.v[j]);
   }
 
+  // ALIGNED: group i to the row in global memory.  STAGED: to a shared-memory copy of the row
+  // (send_row takes it from there), where the last group may reach seven values past the end.
   template <typename T>
   __device__ __forceinline__ void store(T* row, int i, const float (&v)[8]) const {
-    if (L == VECTOR) {
-      if (at(i, 0) < C) store8(row + at(i, 0), v);
-    } else {
+    Raw8<T> r;
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (at(i, j) < C) __stcs(row + unsigned(at(i, j)), from_float<T>(v[j]));
+    for (int j = 0; j < 8; ++j) r.v[j] = from_float<T>(v[j]);
+    if (at(i, 0) >= C) return;
+    const uint4* s = reinterpret_cast<const uint4*>(&r);
+#pragma unroll
+    for (int k = 0; k < int(sizeof(Raw8<T>) / 16); ++k) {
+      if (L == ALIGNED) __stcs(reinterpret_cast<uint4*>(row + at(i, 0)) + k, s[k]);
+      else reinterpret_cast<uint4*>(row + at(i, 0))[k] = s[k];
     }
   }
 
-  // v quantised (VECTOR: rows start at 8-byte boundaries).
+  // The same for v quantised (ALIGNED: rows start at 8-byte boundaries).
   __device__ __forceinline__ void store_quantised(int8_t* row, int i, const float (&v)[8], float inverse) const {
     uint32_t r[8] = {};
     if (inverse != 0.f) {
@@ -178,19 +174,99 @@ struct Spread {
 #pragma unroll
       for (int j = 0; j < 8; ++j) r[j] = __float_as_uint(sum[j]);
     }
-    if (L == VECTOR) {
-      if (at(i, 0) < C) {
-        const uint32_t lo = __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
-        const uint32_t hi = __byte_perm(__byte_perm(r[4], r[5], 0x0040), __byte_perm(r[6], r[7], 0x0040), 0x5410);
-        __stcs(reinterpret_cast<uint2*>(row + at(i, 0)), make_uint2(lo, hi));
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (at(i, j) < C) row[unsigned(at(i, j))] = int8_t(uint8_t(r[j]));
-    }
+    if (at(i, 0) >= C) return;
+    const uint2 q = make_uint2(
+        __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410),
+        __byte_perm(__byte_perm(r[4], r[5], 0x0040), __byte_perm(r[6], r[7], 0x0040), 0x5410));
+    if (L == ALIGNED) __stcs(reinterpret_cast<uint2*>(row + at(i, 0)), q);
+    else *reinterpret_cast<uint2*>(row + at(i, 0)) = q;
   }
 };
+
+// ------------------------------------------------------------------ staged rows
+// Rows that start anywhere: the bytes move in aligned 16-byte granules between global and shared
+// memory, and are shifted by the row's offset (the same for the whole row) between shared memory
+// and registers.  Loads and stores of single values took twice as long (quant_per_token on 4000 x
+// 11007 BF16: 106 us against 51).
+
+// A staged input's room: its granules, and one more that the last shift reads.
+__host__ __device__ constexpr int staged_bytes(long long bytes) { return int((bytes + 15) / 16 * 16 + 48); }
+
+// Starts copying the granules that hold [src, src + bytes) to shared memory.  Bytes of granules that reach
+// outside [begin, end) are loaded singly.
+__device__ __forceinline__ void fetch_row(uint32_t dst, uintptr_t src, int bytes, uintptr_t begin, uintptr_t end, int t,
+                                          int threads) {
+  const uintptr_t first = src & ~uintptr_t(15);
+  const int granules = int((src + bytes + 15 - first) / 16);
+  for (int g = t; g < granules; g += threads) {
+    const uintptr_t at = first + size_t(g) * 16;
+    if (at >= begin && at + 16 <= end) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + g * 16), "l"(at) : "memory");
+    } else {
+      uint32_t w[4] = {};
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (at + e >= begin && at + e < end) w[e / 4] |= uint32_t(*reinterpret_cast<const uint8_t*>(at + e)) << (e % 4 * 8);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sts32(dst + g * 16 + k * 4, w[k]);
+    }
+  }
+}
+__device__ __forceinline__ void fetched() {
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
+}
+
+// Words from byte `offset` (0 to 15, the same for all threads) of the granules at `from` on.
+template <int WORDS>
+__device__ __forceinline__ void shifted_words(uint32_t from, unsigned offset, uint32_t (&out)[WORDS]) {
+  uint32_t w[WORDS + 4];
+#pragma unroll
+  for (int k = 0; k < WORDS / 4 + 1; ++k) {
+    const int4 x = lds128(from + k * 16);
+    w[4 * k] = x.x, w[4 * k + 1] = x.y, w[4 * k + 2] = x.z, w[4 * k + 3] = x.w;
+  }
+#pragma unroll
+  for (int k = 0; k < WORDS + 2; ++k) w[k] = offset & 8 ? w[k + 2] : w[k];
+#pragma unroll
+  for (int k = 0; k < WORDS + 1; ++k) w[k] = offset & 4 ? w[k + 1] : w[k];
+#pragma unroll
+  for (int k = 0; k < WORDS; ++k) out[k] = __funnelshift_r(w[k], w[k + 1], (offset & 3) * 8);
+}
+// Eight values of type T, `index` values into a fetched row.
+template <typename T>
+__device__ __forceinline__ void read_staged(uint32_t row, unsigned offset, int index, float (&v)[8]) {
+  uint32_t w[2 * int(sizeof(T))];
+  shifted_words(row + index * int(sizeof(T)), offset, w);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (sizeof(T) == 4) {
+      v[2 * k] = __uint_as_float(w[2 * k]);
+      v[2 * k + 1] = __uint_as_float(w[2 * k + 1]);
+    } else {
+      const float2 p = unpack2<T>(w[k]);
+      v[2 * k] = p.x;
+      v[2 * k + 1] = p.y;
+    }
+  }
+}
+
+// Writes `bytes` bytes at shared-memory address `from` (16-byte aligned) to dst, whatever its alignment: whole
+// granules, and the bytes of the row's first and last one singly.
+__device__ __forceinline__ void send_row(uintptr_t dst, uint32_t from, int bytes, int t, int threads) {
+  const int head = min(bytes, int(-dst & 15));  // bytes before the first whole granule
+  const int whole = (bytes - head) / 16;
+  for (int g = t; g < whole; g += threads) {
+    uint32_t w[4];
+    shifted_words(from + g * 16, unsigned(head), w);
+    __stcs(reinterpret_cast<uint4*>(dst + head + size_t(g) * 16), make_uint4(w[0], w[1], w[2], w[3]));
+  }
+  const int tail = bytes - head - whole * 16;
+  if (t < head + tail) {  // at most 30
+    const int b = t < head ? t : whole * 16 + t;
+    *reinterpret_cast<uint8_t*>(dst + b) = uint8_t(lds32(from + b / 4 * 4) >> (b % 4 * 8));
+  }
+}
 
 // Reductions over the threads of one row: a warp, or all warps of a block.  `scratch` holds one
 // word per warp and serves one reduction.  The order of the additions is fixed.
@@ -274,7 +350,7 @@ struct RowPlan {
   int rows_per_block = 1;
   int cluster = 1;  // blocks of a row
 };
-inline RowPlan plan_row(int C, int units, int most_threads, int most_blocks) {
+inline RowPlan plan_row(int C, int units, int most_threads, int most_blocks, bool aligned_rows) {
   RowPlan p;
   const int groups = (C + 7) / 8;
   auto threads = [&] { return (groups + 32 * units * p.cluster - 1) / (32 * units * p.cluster) * 32; };
@@ -282,8 +358,21 @@ inline RowPlan plan_row(int C, int units, int most_threads, int most_blocks) {
   if (threads() > most_threads) return p;
   p.units = units;
   p.threads = threads();
-  p.rows_per_block = p.threads == 32 && p.cluster == 1 ? 4 : 1;
+  p.rows_per_block = p.threads == 32 && p.cluster == 1 && aligned_rows ? 4 : 1;
   return p;
+}
+constexpr int SMEM_LIMIT = 232448 - 2048;  // (the kernels' own few words are static)
+// Launches a kernel on staged rows; the attribute is set before every launch that needs it, which
+// costs less than keeping track of devices and kernels.
+template <typename... Params, typename... Args>
+static bool launch_staged(void (*kernel)(Params...), unsigned grid, dim3 block, int bytes, cudaStream_t stream,
+                          Args... args) {
+  if (bytes > 48 * 1024 &&
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  return launch_on_stream(kernel, grid, block, bytes, 1, stream, args...);
 }
 
 }  // namespace row
