@@ -123,6 +123,33 @@ def test_mm_paths_agree(ops, path, shape, out_type):
     assert ops.status() == 0
 
 
+def test_mm_with_less_workspace_than_it_asks_for(ops):
+    """Without the workspace for padded copies the call gathers, and gives the same bits."""
+    from texo_b200 import _lib
+
+    M, N, K = 300, 1001, 2047
+    A, B, sa, sb, bias = mm_inputs(M, N, K, 11)
+    want = ops.mm_int8_per_token(A, B, sa, sb, bias, out_dtype=torch.float32)
+    lib = _lib.load()
+    lib.texo_mm_int8_per_token_force_path(2)  # streaming, which needs the copies here
+    try:
+        asked = lib.texo_mm_int8_per_token_workspace(A.data_ptr(), B.data_ptr(), M, N, K)
+        assert asked == M * 2048 + K * 1008
+        space = torch.full((asked + 16,), 3, dtype=torch.uint8, device="cuda")
+        stream = torch.cuda.current_stream().cuda_stream
+        for pointer, size, path in ((None, 0, 3), (space.data_ptr(), asked - 1, 3), (space.data_ptr() + 1, asked, 3),
+                                    (None, asked, 3), (space.data_ptr(), asked, 2)):
+            got = torch.zeros_like(want)
+            assert lib.texo_mm_int8_solve_per_token(A.data_ptr(), B.data_ptr(), got.data_ptr(), M, N, K, sa.data_ptr(),
+                                                    sb.data_ptr(), bias.data_ptr(), 2, pointer, size, stream) == 0
+            assert torch.equal(got, want)
+            assert lib.texo_mm_int8_per_token_last_path() == path
+            assert path == 2 or bool((space == 3).all())
+    finally:
+        lib.texo_mm_int8_per_token_force_path(0)
+    assert bool((space[asked:] == 3).all())
+
+
 @pytest.mark.parametrize("shape", [(20, 256, 8192), (160, 512, 30000), (3, 100, 4099)])
 def test_mm_extreme_values(ops, shape):
     """All -128 against all -128: the largest dots there are (2^14 K), and their rounding to FP32."""
@@ -269,7 +296,8 @@ def norm_expected(x, r, w, p, gate, eps, scale):
 
 
 NORM_SHAPES = [(1, 1), (1, 8192), (2, 7), (4, 64), (3, 1000), (6, 1001), (600, 96), (514, 264), (700, 512),
-               (512, 1024), (600, 1025), (34, 4096), (520, 4999), (2, 16384), (514, 16384), (4, 16385), (2, 20002)]
+               (512, 1024), (600, 1025), (34, 4096), (520, 4999), (513, 16383), (2, 16384), (514, 16384), (4, 16385),
+               (2, 20002)]
 NORM_TYPES = [(F16, F16, F16), (BF16, F32, BF16), (BF16, BF16, F32), (F32, F32, F32), (F16, F32, F32)]
 
 
@@ -363,7 +391,7 @@ def test_block_norm_rows_that_are_not_finite(ops, C):
 
 # ------------------------------------------------------------------ quantisers
 QUANT_SHAPES = [(1, 1), (1, 5), (16, 8192), (3, 64), (700, 100), (520, 128), (600, 1024), (515, 4999), (33, 16384),
-                (513, 16384), (2, 16385), (3, 28672), (2, 40001)]
+                (513, 16384), (2, 16385), (600, 20001), (3, 28672), (520, 28672), (2, 40001), (515, 65536), (2, 140000)]
 
 
 @pytest.mark.parametrize("shape", QUANT_SHAPES)
@@ -420,6 +448,49 @@ def test_quant_of_unusual_rows(ops, C):
         assert bool((q[row] == value).all()), row
     assert s[0].item() == s[3].item() == s[6].item()
     assert_within(s[4:8], x[4:8, 0].double().abs() / 127, x[4:8, 0].double().abs() / 127 * 1.01 * U)
+
+
+@pytest.mark.parametrize("shape", [(5, 100), (3, 5001), (520, 333), (513, 4096)])
+@pytest.mark.parametrize("shift", [0, 1, 3])
+def test_producers_write_their_outputs_alone(ops, shape, shift):
+    """Outputs inside wider buffers, at addresses aligned to no more than an element: the same values, and
+    nothing around them touched."""
+    N, C = shape
+    x, r, w, p, gt = norm_inputs(N, C, F16, F32, F16, "channel", 5)
+
+    def room(dt):
+        base = torch.full((N * C + 128,), 77, dtype=dt, device="cuda")
+        return base, base[64 + shift:64 + shift + N * C].view(N, C)
+
+    def untouched(base):
+        return bool((base[:64 + shift] == 77).all()) and bool((base[64 + shift + N * C:] == 77).all())
+
+    for call, dt in ((ops.block_norm, torch.float16), (ops.block_norm_quant_per_token, torch.int8)):
+        want = call(x, r, w, 1e-5, post_weight=p, gate=gt)
+        out_base, out = room(dt)
+        z_base, z = room(torch.float32)
+        got = call(x, r, w, 1e-5, post_weight=p, gate=gt, out=out, z_out=z)
+        assert untouched(out_base) and untouched(z_base)
+        if shift == 0:  # (another path may sum in another order)
+            assert all(torch.equal(a, b) for a, b in zip(want, got))
+        y64, dy, z64, dz = norm_expected(x, r, w, p, gt, 1e-5, 1.0)
+        assert_within(z, z64, dz + half_step(z64, torch.float32) * 1.01)
+        if dt == torch.int8:
+            check_quantised(got[0], got[1], y64, dy)
+        else:
+            assert_within(out, y64, dy + half_step(y64, torch.float16) * 1.01)
+    base, out = room(torch.int8)
+    q, s = ops.quant_per_token(x, out=out)
+    want = ops.quant_per_token(x)
+    assert untouched(base) and torch.equal(q, want[0]) and torch.equal(s, want[1])
+    if C % 2 == 0:
+        base = torch.full((N * (C // 2) + 128,), 77, dtype=torch.int8, device="cuda")
+        out = base[64 + shift:64 + shift + N * (C // 2)].view(N, C // 2)
+        for inter in (True, False):
+            q, s = ops.swiglu_quant_per_token(x, interleaved=inter, out=out)
+            want = ops.swiglu_quant_per_token(x, interleaved=inter)
+            assert torch.equal(q, want[0]) and torch.equal(s, want[1])
+            assert bool((base[:64 + shift] == 77).all()) and bool((base[64 + shift + N * (C // 2):] == 77).all())
 
 
 def test_swiglu_of_far_gates(ops):

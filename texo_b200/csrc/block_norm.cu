@@ -261,7 +261,7 @@ static bool launch(const Args& a, cudaStream_t stream) {
   const row::RowPlan r = row::plan_row(a.C, a.N < 512 && a.C <= 8192 ? 1 : 2, 1024, 1, aligned_rows);
   if (r.units == 0) return launch_on_stream(long_row_kernel<X, R, QUANT>, unsigned(a.N), LONG_THREADS, 0, 1, stream, a);
   const dim3 block(r.threads, r.rows_per_block);
-  const unsigned grid = unsigned((a.N + r.rows_per_block - 1) / r.rows_per_block);
+  const unsigned grid = unsigned(((long long)a.N + r.rows_per_block - 1) / r.rows_per_block);
   if (aligned_rows)
     return r.units == 1
                ? launch_on_stream(row_kernel<X, R, QUANT, row::ALIGNED, 1>, grid, block, 0, 1, stream, a)
@@ -277,6 +277,7 @@ static int solve(const Args& a, int x_type, int residual_type, cudaStream_t stre
       (QUANT ? !a.q || !a.scale : !a.y) || (a.gate && a.rows_per_gate <= 0) ||
       (residual_type != x_type && residual_type != row::TYPE_F32))
     return -1;
+  if (a.C > row::MAX_C) return -2;
   if (x_type != row::TYPE_F16 && x_type != row::TYPE_BF16 && x_type != row::TYPE_F32) return -1;
   const bool f32 = residual_type == row::TYPE_F32;
   bool ok;

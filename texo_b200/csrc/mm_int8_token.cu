@@ -22,6 +22,10 @@
 namespace texo {
 namespace i8t {
 
+// Sizes stay this far below 2^31, so that a tile's coordinates past the end do not wrap.
+constexpr int MAX_SIZE = 0x7fffffff - 1024;
+inline int ceil_div(int a, int b) { return int(((long long)a + b - 1) / b); }
+
 struct Scales {
   const float* a;     // [M]
   const float* b;     // [N]
@@ -982,53 +986,66 @@ __global__ void __launch_bounds__(P_THREADS, 1)
 // Copies of A and B whose rows start at 16-byte boundaries, in the caller's workspace: what the
 // gathering kernel does per tile, once per call.  Rows of `width` bytes become rows of `pitch`
 // (the next multiple of 16) bytes; the bytes between are arbitrary (tensor maps end at `width`).
-// A warp moves 512 bytes of a row: four coalesced words per lane, shifted into place with the
-// word that follows.
+// A lane makes sixteen bytes from the two granules that hold them; a warp has four pieces of 512
+// bytes under way.
 struct Pad {
   const uint8_t* from;
   uint8_t* to;
   long long rows;
   int width, pitch;
-  long long pieces() const { return rows * ((pitch + 511) / 512); }
+  __host__ __device__ int per_row() const { return (pitch + 511) / 512; }
+  __host__ __device__ long long pieces() const { return rows * per_row(); }
 };
-constexpr int PAD_THREADS = 256;
+constexpr int PAD_THREADS = 256, PAD_UNROLL = 4;
+// The granule at `at`, of which bytes outside [begin, end) are not read and come back as 0.
+__device__ __forceinline__ uint4 load_granule(uintptr_t at, uintptr_t begin, uintptr_t end) {
+  if (at >= begin && at + 16 <= end) return __ldg(reinterpret_cast<const uint4*>(at));
+  uint32_t w[4] = {};
+#pragma unroll
+  for (int e = 0; e < 16; ++e)
+    if (at + e >= begin && at + e < end) w[e / 4] |= uint32_t(*reinterpret_cast<const uint8_t*>(at + e)) << (e % 4 * 8);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
 __global__ void __launch_bounds__(PAD_THREADS) pad_kernel(const Pad a, const Pad b, long long a_pieces,
                                                           long long pieces) {
   grid_dependency_trigger();
   grid_dependency_wait();
-  const int lane = threadIdx.x % 32;
-  for (long long i = (long long)blockIdx.x * (PAD_THREADS / 32) + threadIdx.x / 32; i < pieces;
-       i += (long long)gridDim.x * (PAD_THREADS / 32)) {
-    const Pad& p = i < a_pieces ? a : b;
-    const long long piece = i < a_pieces ? i : i - a_pieces;
-    const int per_row = (p.pitch + 511) / 512;
-    const long long row = piece / per_row;
-    const int c0 = int(piece % per_row) * 512 + lane * 4;
-    const uintptr_t begin = reinterpret_cast<uintptr_t>(p.from), end = begin + size_t(p.rows) * p.width;
-    const uintptr_t src = begin + size_t(row) * p.width + c0;
-    const uintptr_t word = src & ~uintptr_t(3);
-    const unsigned bits = unsigned(src & 3) * 8;
-    uint32_t w[4][2];
-    if (word >= begin && word + 3 * 128 + 8 <= end) {
+  const long long warps = (long long)gridDim.x * (PAD_THREADS / 32);
+  for (long long first = (long long)blockIdx.x * (PAD_THREADS / 32) + threadIdx.x / 32; first < pieces;
+       first += warps * PAD_UNROLL) {
+    uint4 lo[PAD_UNROLL], hi[PAD_UNROLL];
+    uint8_t* to[PAD_UNROLL];
+    unsigned offset[PAD_UNROLL];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        w[j][0] = __ldg(reinterpret_cast<const unsigned int*>(word + j * 128));
-        w[j][1] = __ldg(reinterpret_cast<const unsigned int*>(word + j * 128 + 4));
-      }
-    } else {
-      for (int j = 0; j < 4; ++j)
-        for (int h = 0; h < 2; ++h) {
-          w[j][h] = 0;
-          for (int e = 0; e < 4; ++e) {
-            const uintptr_t at = word + j * 128 + h * 4 + e;
-            if (at >= begin && at < end) w[j][h] |= uint32_t(*reinterpret_cast<const uint8_t*>(at)) << (8 * e);
-          }
-        }
+    for (int u = 0; u < PAD_UNROLL; ++u) {
+      const long long i = first + u * warps;
+      to[u] = nullptr;
+      if (i >= pieces) continue;
+      const bool in_a = i < a_pieces;
+      const Pad& p = in_a ? a : b;
+      const long long piece = in_a ? i : i - a_pieces, row = piece / p.per_row();
+      const int c = int(piece - row * p.per_row()) * 512 + int(threadIdx.x % 32) * 16;
+      if (c >= p.pitch) continue;
+      const uintptr_t begin = reinterpret_cast<uintptr_t>(p.from), end = begin + size_t(p.rows) * p.width;
+      const uintptr_t src = begin + size_t(row) * p.width + c;
+      to[u] = p.to + size_t(row) * p.pitch + c;
+      offset[u] = unsigned(src & 15);
+      lo[u] = load_granule(floor16(src), begin, end);
+      hi[u] = load_granule(floor16(src) + 16, begin, end);
     }
-    uint32_t* to = reinterpret_cast<uint32_t*>(p.to + size_t(row) * p.pitch + c0);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (c0 + j * 128 < p.pitch) to[j * 32] = __funnelshift_r(w[j][0], w[j][1], bits);
+    for (int u = 0; u < PAD_UNROLL; ++u) {
+      if (!to[u]) continue;
+      uint32_t w[8] = {lo[u].x, lo[u].y, lo[u].z, lo[u].w, hi[u].x, hi[u].y, hi[u].z, hi[u].w};
+#pragma unroll
+      for (int j = 0; j < 6; ++j) w[j] = offset[u] & 8 ? w[j + 2] : w[j];
+#pragma unroll
+      for (int j = 0; j < 5; ++j) w[j] = offset[u] & 4 ? w[j + 1] : w[j];
+      const unsigned bits = (offset[u] & 3) * 8;
+      *reinterpret_cast<uint4*>(to[u]) =
+          make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
+                     __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+    }
   }
 }
 
@@ -1050,7 +1067,7 @@ static bool launch_generic(const int8_t* A, const int8_t* B, Y* out, int M, int 
   constexpr int ROWS = 65535 * GT;
   for (int m0 = 0; m0 < M; m0 += ROWS) {
     const int rows = std::min(M - m0, ROWS);
-    const dim3 grid((N + GT - 1) / GT, (rows + GT - 1) / GT);
+    const dim3 grid(ceil_div(N, GT), ceil_div(rows, GT));
     const Scales part = {s.a + m0, s.b, s.bias};
     generic_kernel<Y><<<grid, G_THREADS, 0, stream>>>(A + size_t(m0) * K, B, out + size_t(m0) * N, rows, N, K, part);
     ++launch_counter();
@@ -1116,33 +1133,39 @@ static DeviceSetup& device_setup(DeviceCtx& ctx) {
   return d;
 }
 
-// The choice between the paths is by estimated time in microseconds.  The constants are fits to
-// measurements on B200 (kernels back to back, operands from HBM):
+// The choice between the paths, and of R and c, is by estimated time in microseconds.  The constants
+// are fits to measurements on B200 (kernels back to back, operands from HBM):
 //   stream, per k block of 128: 0.42 + 0.0009 R, or its 32 KiB of B at 6.2 TB/s over all CTAs
 //   gather, per k block: 1.15 up to R = 32, then 1.4 (64) and 1.9 (128): shared-memory bandwidth
-//   either, per call: 3.2 (c = 1) or 4.7, and 0.045 R for the drain
+//   either, per round of tiles: 0.3 (c = 1) or 2, per call: 2.2 or 2.7, and 0.045 R for the drain
+//     (0.065 R where rows of Y are not multiples of eight)
 //   pair, per k block 0.33 (0.42 once all SMs run: power), per call 7, per round of tiles 1
-//   padding: 2.5 and twice the operand's bytes at 5 TB/s
+//   padding: 2.5 and twice the operand's bytes at 4.2 TB/s
+// E.g. 512 x 512 x 1024: streaming at R = 16, 32, 128 6.5, 7.3, 12 us, pairs 10.7; 256 x 4096 x
+// 4096: 17.0 against 19.7; 1024 x 4096 x 4096: 25 against 19.9.
 struct StreamPlan {
   int R = 0, cluster = 0, clusters = 0, m_tiles = 0, tiles = 0;
   double us = 1e30;
 };
 static StreamPlan plan_stream(const DeviceSetup& d, bool gather, int M, int N, int K) {
   StreamPlan best;
-  const int r = M <= 16 ? 0 : M <= 32 ? 1 : M <= 64 ? 2 : 3;
-  const int R = R_CHOICES[r];
-  const long long m_tiles = (M + R - 1) / R, tiles = m_tiles * ((N + S_TILE_N - 1) / S_TILE_N);
   const int num_kb = (K + S_BK - 1) / S_BK;
-  if (tiles > 0x3fffffff) return best;
-  for (int c = 1; c <= S_MAX_CLUSTER && c <= num_kb; ++c) {
-    const int held = d.clusters[gather][r][c];
-    if (held <= 0) continue;
-    const int clusters = int(std::min<long long>(tiles, held));
-    const double rounds = double((tiles + clusters - 1) / clusters);
-    const double block = gather ? (R <= 32 ? 1.15 : R == 64 ? 1.4 : 1.9)
-                                : std::max(0.42 + 0.0009 * R, 32768.0 * clusters * c / double(m_tiles) / 6.2e6);
-    const double us = rounds * ((num_kb + c - 1) / c * block + (c > 1 ? 2 : 0.3)) + (c > 1 ? 2.7 : 2.9) + 0.045 * R;
-    if (us < best.us) best = {R, c, clusters, int(m_tiles), int(tiles), us};
+  for (int r = 0; r < 4; ++r) {
+    const int R = R_CHOICES[r];
+    const long long m_tiles = ceil_div(M, R), tiles = m_tiles * ceil_div(N, S_TILE_N);
+    if (tiles > 0x3fffffff) continue;
+    for (int c = 1; c <= S_MAX_CLUSTER && c <= num_kb; ++c) {
+      const int held = d.clusters[gather][r][c];
+      if (held <= 0) continue;
+      const int clusters = int(std::min<long long>(tiles, held));
+      const double rounds = double((tiles + clusters - 1) / clusters);
+      const double block = gather ? (R <= 32 ? 1.15 : R == 64 ? 1.4 : 1.9)
+                                  : std::max(0.42 + 0.0009 * R, 32768.0 * clusters * c / double(m_tiles) / 6.2e6);
+      const double us = rounds * ((num_kb + c - 1) / c * block + (c > 1 ? 2 : 0.3)) + (c > 1 ? 2.7 : 2.2) +
+                        (N % 8 == 0 ? 0.045 : 0.065) * R;
+      if (us < best.us) best = {R, c, clusters, int(m_tiles), int(tiles), us};
+    }
+    if (M <= R) break;  // a larger R only pads
   }
   return best;
 }
@@ -1164,12 +1187,12 @@ static Route choose_route(const DeviceSetup& d, int M, int N, int K, bool a_ok, 
   if (K <= 0 || K >= (1 << 17) || force == PATH_GENERIC) return best;
   const long long pad = pad_bytes(M, N, K, !a_ok, !b_ok);
   if (pad <= workspace && force != PATH_STREAM_GATHER) {
-    const double pad_us = pad ? 2.5 + 2.0 * double(pad) / 5e6 : 0;
+    const double pad_us = pad ? 2.5 + 2.0 * double(pad) / 4.2e6 : 0;
     if (force != PATH_PAIR) {
       const StreamPlan plan = plan_stream(d, false, M, N, K);
       if (plan.cluster > 0) best = {PATH_STREAM, !a_ok, !b_ok, plan, plan.us + pad_us};
     }
-    const long long tiles = (long long)((M + 255) / 256) * ((N + 255) / 256);
+    const long long tiles = (long long)ceil_div(M, 256) * ceil_div(N, 256);
     if (d.pairs > 0 && tiles <= 0x3fffffff && force != PATH_STREAM) {
       const double rounds = double((tiles + d.pairs - 1) / d.pairs);
       const double us = 7 + rounds * ((K + 127) / 128 * (rounds > 2 ? 0.42 : 0.33) + 1) + pad_us;
@@ -1221,7 +1244,7 @@ static bool launch_pair(DeviceCtx& ctx, const DeviceSetup& d, const Operand& A, 
       (tma_out && !make_tensor_map_2d(&map_y, TYPE, sizeof(Y), out, M, N, size_t(N) * sizeof(Y), 32, 128 / sizeof(Y),
                                       CU_TENSOR_MAP_SWIZZLE_128B)))
     return false;
-  const PairShape p = {M, N, K, (M + 255) / 256, (N + 255) / 256, i8::raster_group_rows(K)};
+  const PairShape p = {M, N, K, ceil_div(M, 256), ceil_div(N, 256), i8::raster_group_rows(K)};
   const int clusters = std::min(p.tiles_m * p.tiles_n, d.pairs);
   return tma_out ? launch_on_stream(pair_kernel<Y, true>, 2 * clusters, P_THREADS, P_SMEM_BYTES, 2, stream, map_a,
                                    map_b, map_y, out, s, p, ctx.status)
@@ -1286,7 +1309,7 @@ extern "C" long long texo_mm_int8_per_token_workspace(const int8_t* A, const int
   using namespace texo;
   const bool a_ok = i8t::tma_can_move(A, K), b_ok = i8t::tma_can_move(B, N);
   int device;
-  if (M <= 0 || N <= 0 || K <= 0 || (a_ok && b_ok) || !device_ctx_entry(device).ready || !i8t::setups[device].ready)
+  if (M <= 0 || N <= 0 || K <= 0 || M > i8t::MAX_SIZE || N > i8t::MAX_SIZE || (a_ok && b_ok) || !device_ctx_entry(device).ready || !i8t::setups[device].ready)
     return 0;
   const i8t::Route route =
       i8t::choose_route(i8t::setups[device], M, N, K, a_ok, b_ok, 0x7fffffffffffffffLL, i8t::forced_path());
@@ -1298,6 +1321,7 @@ extern "C" int texo_mm_int8_solve_per_token(const int8_t* A, const int8_t* B, vo
                                             int out_type, void* workspace, long long workspace_bytes, void* stream) {
   using namespace texo;
   if (M <= 0 || N <= 0 || K < 0 || !Y || !scale_A || !scale_B || (K > 0 && (!A || !B))) return -1;
+  if (M > i8t::MAX_SIZE || N > i8t::MAX_SIZE || K > i8t::MAX_SIZE) return -2;
   const i8t::Scales s = {scale_A, scale_B, bias};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (out_type) {

@@ -206,6 +206,7 @@ template <int FORM>
 static int solve(const Args& a, int x_type, cudaStream_t stream) {
   const long long width = FORM == PLAIN ? a.C : 2LL * a.C;
   if (a.N <= 0 || a.C <= 0 || a.stride < width || !a.x || !a.q || !a.scale) return -1;
+  if (width > row::MAX_C) return -2;
   if (x_type != row::TYPE_F16 && x_type != row::TYPE_BF16 && x_type != row::TYPE_F32) return -1;
   const bool ok = x_type == row::TYPE_F16    ? launch<__half, FORM>(a, stream)
                   : x_type == row::TYPE_BF16 ? launch<__nv_bfloat16, FORM>(a, stream)

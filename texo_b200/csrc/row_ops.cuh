@@ -342,6 +342,7 @@ __device__ __forceinline__ float token_inverse(float amax) {
 }
 
 // ------------------------------------------------------------------- host side
+constexpr int MAX_C = 0x7fffffff - 4096;  // positions a block's width past the end do not wrap
 // How rows are laid over threads and blocks: `units` groups of eight per thread at most, blocks of
 // at most `most_threads`, clusters of at most `most_blocks`.
 struct RowPlan {
