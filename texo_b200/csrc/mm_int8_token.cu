@@ -986,17 +986,15 @@ __global__ void __launch_bounds__(P_THREADS, 1)
 // Copies of A and B whose rows start at 16-byte boundaries, in the caller's workspace: what the
 // gathering kernel does per tile, once per call.  Rows of `width` bytes become rows of `pitch`
 // (the next multiple of 16) bytes; the bytes between are arbitrary (tensor maps end at `width`).
-// A lane makes sixteen bytes from the two granules that hold them; a warp has four pieces of 512
-// bytes under way.
+// A lane makes sixteen bytes from the two granules that hold them; a warp takes 2 KiB of a row,
+// four pieces at once, and a block eight rows.
 struct Pad {
   const uint8_t* from;
   uint8_t* to;
-  long long rows;
-  int width, pitch;
-  __host__ __device__ int per_row() const { return (pitch + 511) / 512; }
-  __host__ __device__ long long pieces() const { return rows * per_row(); }
+  int rows, width, pitch;
+  int parts() const { return (pitch + 2047) / 2048; }
 };
-constexpr int PAD_THREADS = 256, PAD_UNROLL = 4;
+constexpr int PAD_ROWS = 8, PAD_THREADS = PAD_ROWS * 32;
 // The granule at `at`, of which bytes outside [begin, end) are not read and come back as 0.
 __device__ __forceinline__ uint4 load_granule(uintptr_t at, uintptr_t begin, uintptr_t end) {
   if (at >= begin && at + 16 <= end) return __ldg(reinterpret_cast<const uint4*>(at));
@@ -1006,45 +1004,39 @@ __device__ __forceinline__ uint4 load_granule(uintptr_t at, uintptr_t begin, uin
     if (at + e >= begin && at + e < end) w[e / 4] |= uint32_t(*reinterpret_cast<const uint8_t*>(at + e)) << (e % 4 * 8);
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
-__global__ void __launch_bounds__(PAD_THREADS) pad_kernel(const Pad a, const Pad b, long long a_pieces,
-                                                          long long pieces) {
+// blockIdx = (part of the row, rows, operand).
+__global__ void __launch_bounds__(PAD_THREADS) pad_kernel(const Pad a, const Pad b) {
   grid_dependency_trigger();
+  const Pad& p = blockIdx.z == 0 ? a : b;
+  const int c0 = int(blockIdx.x) * 2048 + int(threadIdx.x % 32) * 16;
+  const uintptr_t begin = reinterpret_cast<uintptr_t>(p.from), end = begin + size_t(p.rows) * p.width;
   grid_dependency_wait();
-  const long long warps = (long long)gridDim.x * (PAD_THREADS / 32);
-  for (long long first = (long long)blockIdx.x * (PAD_THREADS / 32) + threadIdx.x / 32; first < pieces;
-       first += warps * PAD_UNROLL) {
-    uint4 lo[PAD_UNROLL], hi[PAD_UNROLL];
-    uint8_t* to[PAD_UNROLL];
-    unsigned offset[PAD_UNROLL];
+  if (int(blockIdx.x) * 2048 >= p.pitch) return;
+  for (long long row = (long long)blockIdx.y * PAD_ROWS + threadIdx.x / 32; row < p.rows;
+       row += (long long)gridDim.y * PAD_ROWS) {
+    const uintptr_t src = begin + size_t(row) * p.width + c0;
+    const unsigned offset = unsigned(src & 15);
+    uint4 lo[4], hi[4];
 #pragma unroll
-    for (int u = 0; u < PAD_UNROLL; ++u) {
-      const long long i = first + u * warps;
-      to[u] = nullptr;
-      if (i >= pieces) continue;
-      const bool in_a = i < a_pieces;
-      const Pad& p = in_a ? a : b;
-      const long long piece = in_a ? i : i - a_pieces, row = piece / p.per_row();
-      const int c = int(piece - row * p.per_row()) * 512 + int(threadIdx.x % 32) * 16;
-      if (c >= p.pitch) continue;
-      const uintptr_t begin = reinterpret_cast<uintptr_t>(p.from), end = begin + size_t(p.rows) * p.width;
-      const uintptr_t src = begin + size_t(row) * p.width + c;
-      to[u] = p.to + size_t(row) * p.pitch + c;
-      offset[u] = unsigned(src & 15);
-      lo[u] = load_granule(floor16(src), begin, end);
-      hi[u] = load_granule(floor16(src) + 16, begin, end);
+    for (int u = 0; u < 4; ++u) {
+      if (c0 + u * 512 < p.pitch) {
+        lo[u] = load_granule(floor16(src) + u * 512, begin, end);
+        hi[u] = load_granule(floor16(src) + u * 512 + 16, begin, end);
+      }
     }
 #pragma unroll
-    for (int u = 0; u < PAD_UNROLL; ++u) {
-      if (!to[u]) continue;
-      uint32_t w[8] = {lo[u].x, lo[u].y, lo[u].z, lo[u].w, hi[u].x, hi[u].y, hi[u].z, hi[u].w};
+    for (int u = 0; u < 4; ++u) {
+      if (c0 + u * 512 < p.pitch) {
+        uint32_t w[8] = {lo[u].x, lo[u].y, lo[u].z, lo[u].w, hi[u].x, hi[u].y, hi[u].z, hi[u].w};
 #pragma unroll
-      for (int j = 0; j < 6; ++j) w[j] = offset[u] & 8 ? w[j + 2] : w[j];
+        for (int j = 0; j < 6; ++j) w[j] = offset & 8 ? w[j + 2] : w[j];
 #pragma unroll
-      for (int j = 0; j < 5; ++j) w[j] = offset[u] & 4 ? w[j + 1] : w[j];
-      const unsigned bits = (offset[u] & 3) * 8;
-      *reinterpret_cast<uint4*>(to[u]) =
-          make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
-                     __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+        for (int j = 0; j < 5; ++j) w[j] = offset & 4 ? w[j + 1] : w[j];
+        const unsigned bits = (offset & 3) * 8;
+        *reinterpret_cast<uint4*>(p.to + size_t(row) * p.pitch + c0 + u * 512) =
+            make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
+                       __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+      }
     }
   }
 }
@@ -1136,11 +1128,11 @@ static DeviceSetup& device_setup(DeviceCtx& ctx) {
 // The choice between the paths, and of R and c, is by estimated time in microseconds.  The constants
 // are fits to measurements on B200 (kernels back to back, operands from HBM):
 //   stream, per k block of 128: 0.42 + 0.0009 R, or its 32 KiB of B at 6.2 TB/s over all CTAs
-//   gather, per k block: 1.15 up to R = 32, then 1.4 (64) and 1.9 (128): shared-memory bandwidth
+//   gather, per k block: 1.3 up to R = 32, then 1.8 (64) and 2.8 (128): shared-memory bandwidth
 //   either, per round of tiles: 0.3 (c = 1) or 2, per call: 2.2 or 2.7, and 0.045 R for the drain
 //     (0.065 R where rows of Y are not multiples of eight)
 //   pair, per k block 0.33 (0.42 once all SMs run: power), per call 7, per round of tiles 1
-//   padding: 2.5 and twice the operand's bytes at 4.2 TB/s
+//   padding: 2.5 and twice the operand's bytes at 5 TB/s
 // E.g. 512 x 512 x 1024: streaming at R = 16, 32, 128 6.5, 7.3, 12 us, pairs 10.7; 256 x 4096 x
 // 4096: 17.0 against 19.7; 1024 x 4096 x 4096: 25 against 19.9.
 struct StreamPlan {
@@ -1159,7 +1151,7 @@ static StreamPlan plan_stream(const DeviceSetup& d, bool gather, int M, int N, i
       if (held <= 0) continue;
       const int clusters = int(std::min<long long>(tiles, held));
       const double rounds = double((tiles + clusters - 1) / clusters);
-      const double block = gather ? (R <= 32 ? 1.15 : R == 64 ? 1.4 : 1.9)
+      const double block = gather ? (R <= 32 ? 1.3 : R == 64 ? 1.8 : 2.8)
                                   : std::max(0.42 + 0.0009 * R, 32768.0 * clusters * c / double(m_tiles) / 6.2e6);
       const double us = rounds * ((num_kb + c - 1) / c * block + (c > 1 ? 2 : 0.3)) + (c > 1 ? 2.7 : 2.2) +
                         (N % 8 == 0 ? 0.045 : 0.065) * R;
@@ -1187,7 +1179,7 @@ static Route choose_route(const DeviceSetup& d, int M, int N, int K, bool a_ok, 
   if (K <= 0 || K >= (1 << 17) || force == PATH_GENERIC) return best;
   const long long pad = pad_bytes(M, N, K, !a_ok, !b_ok);
   if (pad <= workspace && force != PATH_STREAM_GATHER) {
-    const double pad_us = pad ? 2.5 + 2.0 * double(pad) / 4.2e6 : 0;
+    const double pad_us = pad ? 2.5 + 2.0 * double(pad) / 5e6 : 0;
     if (force != PATH_PAIR) {
       const StreamPlan plan = plan_stream(d, false, M, N, K);
       if (plan.cluster > 0) best = {PATH_STREAM, !a_ok, !b_ok, plan, plan.us + pad_us};
@@ -1253,22 +1245,23 @@ static bool launch_pair(DeviceCtx& ctx, const DeviceSetup& d, const Operand& A, 
 }
 
 // Makes the padded copies in the workspace and points the operands at them.
-static bool launch_pad(const DeviceCtx& ctx, const Route& route, Operand& A, Operand& B, int M, int N, int K,
+static bool launch_pad(const Route& route, Operand& A, Operand& B, int M, int N, int K,
                        void* workspace, cudaStream_t stream) {
   uint8_t* to = static_cast<uint8_t*>(workspace);
-  Pad a = {}, b = {};
+  Pad pads[2] = {};
+  int n = 0;
   if (route.pad_a) {
-    a = {reinterpret_cast<const uint8_t*>(A.p), to, M, K, padded(K)};
+    pads[n++] = {reinterpret_cast<const uint8_t*>(A.p), to, M, K, padded(K)};
     A = {reinterpret_cast<int8_t*>(to), padded(K)};
     to += size_t(M) * padded(K);
   }
   if (route.pad_b) {
-    b = {reinterpret_cast<const uint8_t*>(B.p), to, K, N, padded(N)};
+    pads[n++] = {reinterpret_cast<const uint8_t*>(B.p), to, K, N, padded(N)};
     B = {reinterpret_cast<int8_t*>(to), padded(N)};
   }
-  const long long a_pieces = a.pieces(), pieces = a_pieces + b.pieces();
-  const int grid = int(std::min<long long>((pieces + PAD_THREADS / 32 - 1) / (PAD_THREADS / 32), ctx.sm_count * 8));
-  return launch_on_stream(pad_kernel, grid, PAD_THREADS, 0, 1, stream, a, b, a_pieces, pieces);
+  const int rows = std::max(pads[0].rows, pads[1].rows);
+  const dim3 grid(std::max(pads[0].parts(), pads[1].parts()), std::min(ceil_div(rows, PAD_ROWS), 65535), n);
+  return launch_on_stream(pad_kernel, grid, PAD_THREADS, 0, 1, stream, pads[0], pads[1]);
 }
 
 static bool tma_can_move(const int8_t* p, int width) {
@@ -1287,7 +1280,7 @@ static int solve(const int8_t* A, const int8_t* B, Y* out, int M, int N, int K, 
     const Route route = choose_route(d, M, N, K, tma_can_move(A, K), tma_can_move(B, N), workspace_bytes, forced_path());
     Operand a = {A, K}, b = {B, N};
     if (route.path != PATH_GENERIC &&
-        (!(route.pad_a || route.pad_b) || launch_pad(ctx, route, a, b, M, N, K, workspace, stream)) &&
+        (!(route.pad_a || route.pad_b) || launch_pad(route, a, b, M, N, K, workspace, stream)) &&
         (route.path == PATH_PAIR     ? launch_pair(ctx, d, a, b, out, M, N, K, s, stream)
          : route.path == PATH_STREAM ? launch_stream<Y, false>(ctx, route.stream, a, b, out, M, N, K, s, stream)
                                      : launch_stream<Y, true>(ctx, route.stream, a, b, out, M, N, K, s, stream))) {

@@ -198,10 +198,18 @@ __device__ __forceinline__ void fetch_row(uint32_t dst, uintptr_t src, int bytes
                                           int threads) {
   const uintptr_t first = src & ~uintptr_t(15);
   const int granules = int((src + bytes + 15 - first) / 16);
+  auto copy = [&](int g, uintptr_t at) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + g * 16), "l"(at) : "memory");
+  };
+  if (first >= begin && first + size_t(granules) * 16 <= end) {
+    uintptr_t at = first + size_t(t) * 16;
+    for (int g = t; g < granules; g += threads, at += size_t(threads) * 16) copy(g, at);
+    return;
+  }
   for (int g = t; g < granules; g += threads) {
     const uintptr_t at = first + size_t(g) * 16;
     if (at >= begin && at + 16 <= end) {
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + g * 16), "l"(at) : "memory");
+      copy(g, at);
     } else {
       uint32_t w[4] = {};
 #pragma unroll
