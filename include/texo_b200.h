@@ -346,8 +346,8 @@ int texo_block_norm_solve(const void* x, const void* residual, const void* weigh
                           int gate_rows, int gate_per_channel, float eps, float residual_scale,
                           int x_type, int residual_type, int weights_f32, void* stream);
 /* The same with y quantised per token: scale [N] FP32, q [N,C] int8,
- *   scale = max(max_j |y|, 2^-100) / 127,   q = rint(y * (127 / max(max_j |y|, 2^-100)))
- * (within [-127, 127]).  A row whose y holds a NaN or an infinity gets scale NaN and q = 0. */
+ *   scale = max(max_j |y|, 2^-100) / 127,   q = rint(y / scale)
+ * (within [-127, 127]; both quotients rounded to FP32).  A row whose y holds a NaN or an infinity gets scale NaN and q = 0. */
 int texo_block_norm_quant_solve(const void* x, const void* residual, const void* weight,
                                 const void* post_weight, const void* gate, int8_t* q, float* scale,
                                 void* z, int N, int C, int gate_rows, int gate_per_channel, float eps,

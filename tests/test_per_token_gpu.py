@@ -320,9 +320,9 @@ def test_block_norm_matches_64_bits(ops, shape, types, post, gate):
 
 
 def check_quantised(q, s, y, dy):
-    """scale: the row maximum's error, one division.  q: rint of y * (127 / maximum), where y, the
-    maximum (their errors dy) and two roundings move the argument; an argument next to a tie may
-    round either way."""
+    """scale: the row maximum's error, one division.  q: rint of y / scale, where y, the maximum
+    (their errors dy) and two roundings (scale's, the quotient's) move the argument; an argument
+    next to a tie may round either way."""
     assert q.dtype == torch.int8 and s.dtype == torch.float32
     amax = y.abs().amax(dim=1)
     damax = dy.amax(dim=1)
@@ -401,6 +401,23 @@ def test_quant_matches_64_bits(ops, shape, x_type):
     x = (torch.randn(*shape, generator=g, device="cuda") * 3).to(dtype(x_type))
     q, s = ops.quant_per_token(x)
     check_quantised(q, s, x.double(), torch.zeros_like(x, dtype=torch.float64))
+
+
+@pytest.mark.parametrize("shape", [(64, 512), (3, 8192), (515, 1001), (2, 140000)])
+@pytest.mark.parametrize("x_type", [F16, BF16])
+def test_quant_of_ties(ops, shape, x_type):
+    """Values of few bits lie half way between two multiples of the scale often: the quotient in FP32
+    decides, ties to even, as elementary operations do it."""
+    g = generator(9)
+    x = torch.randint(-254, 255, shape, generator=g, device="cuda").to(dtype(x_type))
+    x[:, 0] = 254
+    x[0] *= 0.37
+    q, s = ops.quant_per_token(x)
+    want = x.float().abs().amax(dim=1) / 127
+    assert torch.equal(s, want)
+    t = x.float() / want[:, None]
+    assert torch.equal(q.float(), torch.round(t))
+    assert bool(((t[1:] % 1).abs() == 0.5).any())
 
 
 @pytest.mark.parametrize("shape", QUANT_SHAPES)

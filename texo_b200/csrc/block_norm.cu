@@ -112,10 +112,10 @@ __device__ __forceinline__ void finish(const Args& a, int n, X* y, int8_t* q, co
   }
   if (QUANT) {
     amax = row::row_max(amax, max_scratch, s.t, warps);
-    if (s.t == 0) a.scale[n] = row::token_scale(amax);
-    const float inverse = row::token_inverse(amax);
+    const row::TokenScale scale = row::token_scale(amax);
+    if (s.t == 0) a.scale[n] = scale.scale;
 #pragma unroll
-    for (int i = 0; i < UNITS; ++i) s.store_quantised(q, i, v[i], inverse);
+    for (int i = 0; i < UNITS; ++i) s.store_quantised(q, i, v[i], scale);
   }
 }
 
@@ -229,20 +229,20 @@ __global__ void __launch_bounds__(LONG_THREADS) long_row_kernel(const Args a) {
     sum += v * v;
   }
   const float inv = rsqrtf(row::row_sum(sum, scratch.sum, threadIdx.x, WARPS) / float(C) + a.eps);
-  float inverse = 0.f;
+  row::TokenScale scale = {0.f, 0.f, 0.f};
   if (QUANT) {
     float amax = 0.f;
     for (int c = threadIdx.x; c < C; c += LONG_THREADS) amax = row::max_abs(amax, z_at(c) * (inv * weight(a.weight, c)));
     amax = row::row_max(amax, scratch.max, threadIdx.x, WARPS);
-    if (threadIdx.x == 0) a.scale[n] = row::token_scale(amax);
-    inverse = row::token_inverse(amax);
+    scale = row::token_scale(amax);
+    if (threadIdx.x == 0) a.scale[n] = scale.scale;
   }
   for (int c = threadIdx.x; c < C; c += LONG_THREADS) {
     const float z = z_at(c);
     const float y = z * (inv * weight(a.weight, c));
     static_cast<R*>(a.z)[at + c] = row::from_float<R>(z);
     if (QUANT)
-      a.q[at + c] = row::quantise(y, inverse);
+      a.q[at + c] = row::quantise(y, scale);
     else
       static_cast<X*>(a.y)[at + c] = row::from_float<X>(y);
   }

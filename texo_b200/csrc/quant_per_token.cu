@@ -97,9 +97,19 @@ __device__ __forceinline__ void read_y(uint32_t first, unsigned offset, uint32_t
   s.mask(i, y);  // (what lies past the row's end is arbitrary)
 }
 
+// Threads of a block at most, and such blocks that an SM has to hold for their latencies to overlap:
+// with two groups per thread in 40 registers instead of 32, 4096 x 28672 interleaved pairs took
+// 148 us instead of 131.
+__host__ __device__ constexpr int block_limit(row::Layout layout, int units) {
+  return layout == row::STAGED || units < 4 ? 1024 : 512;
+}
+__host__ __device__ constexpr int blocks_per_sm(row::Layout layout, int units) {
+  return layout == row::STAGED || units == 1 ? 1 : 2;
+}
+
 // A block, a warp or (blocks > 1) a cluster per row.  blockDim = (threads, rows of the block).
 template <typename X, int FORM, row::Layout L, int UNITS>
-__global__ void __launch_bounds__(UNITS == 4 && L == row::ALIGNED ? 512 : 1024) row_kernel(const Args a, int blocks) {
+__global__ void __launch_bounds__(block_limit(L, UNITS), blocks_per_sm(L, UNITS)) row_kernel(const Args a, int blocks) {
   __shared__ unsigned scratch[row::MAX_WARPS], maxima[row::MAX_CLUSTER];
   grid_dependency_trigger();
   row::cluster_started(blocks);
@@ -138,10 +148,10 @@ __global__ void __launch_bounds__(UNITS == 4 && L == row::ALIGNED ? 512 : 1024) 
     for (int j = 0; j < 8; ++j) amax = row::max_abs(amax, y[i][j]);
   }
   amax = row::cluster_max(amax, scratch, t, threads / 32, maxima, blocks);
-  if (s.t == 0) a.scale[n] = row::token_scale(amax);
-  const float inverse = row::token_inverse(amax);
+  const row::TokenScale scale = row::token_scale(amax);
+  if (s.t == 0) a.scale[n] = scale.scale;
 #pragma unroll
-  for (int i = 0; i < UNITS; ++i) s.store_quantised(q, i, y[i], inverse);
+  for (int i = 0; i < UNITS; ++i) s.store_quantised(q, i, y[i], scale);
   if constexpr (L == row::STAGED) {
     __syncthreads();
     row::send_row(reinterpret_cast<uintptr_t>(a.q + size_t(n) * a.C), smem_u32(q), a.C, t, threads);
@@ -166,10 +176,10 @@ __global__ void __launch_bounds__(LONG_THREADS) long_row_kernel(const Args a) {
   float amax = 0.f;
   for (int c = threadIdx.x; c < a.C; c += LONG_THREADS) amax = row::max_abs(amax, y_at(c));
   amax = row::row_max(amax, scratch, threadIdx.x, LONG_THREADS / 32);
-  if (threadIdx.x == 0) a.scale[n] = row::token_scale(amax);
-  const float inverse = row::token_inverse(amax);
+  const row::TokenScale scale = row::token_scale(amax);
+  if (threadIdx.x == 0) a.scale[n] = scale.scale;
   int8_t* q = a.q + size_t(n) * a.C;
-  for (int c = threadIdx.x; c < a.C; c += LONG_THREADS) q[c] = row::quantise(y_at(c), inverse);
+  for (int c = threadIdx.x; c < a.C; c += LONG_THREADS) q[c] = row::quantise(y_at(c), scale);
 }
 
 template <typename X, int FORM>
@@ -181,7 +191,7 @@ static bool launch(const Args& a, cudaStream_t stream) {
     const int bytes = a.C <= 32768 ? a.C * int(sizeof(X)) * (FORM == SWIGLU_INTERLEAVED ? 2 : 1) : 0;
     const int room = row::staged_bytes(bytes) * (FORM == SWIGLU_HALVES ? 2 : 1);
     // (4000 x 11007 BF16: 85 / 51 us for two / four groups per thread)
-    const row::RowPlan r = row::plan_row(a.C, a.N < 512 && a.C <= 8192 ? 1 : 4, 1024, 1, false);
+    const row::RowPlan r = row::plan_row(a.C, a.N < 512 && a.C <= 8192 ? 1 : 4, block_limit(row::STAGED, 4), 1, false);
     if (r.units == 0 || room > row::SMEM_LIMIT) return launch_long();
     auto rows = [&](auto* kernel) { return row::launch_staged(kernel, unsigned(a.N), dim3(r.threads), room, stream, a, 1); };
     return r.units == 1 ? rows(row_kernel<X, FORM, row::STAGED, 1>) : rows(row_kernel<X, FORM, row::STAGED, 4>);
@@ -190,9 +200,9 @@ static bool launch(const Args& a, cudaStream_t stream) {
   // 60 / 41 / 35 us for one / two / four), or two where 16-bit pairs are interleaved, whose groups
   // are twice as wide (4096 x 11008: 45 / 50 us for two / four).
   const bool wide = FORM == SWIGLU_INTERLEAVED && sizeof(X) == 2;
-  const row::RowPlan r = a.N < 512 ? row::plan_row(a.C, 1, 1024, row::MAX_CLUSTER, true)
+  const row::RowPlan r = a.N < 512 ? row::plan_row(a.C, 1, block_limit(row::ALIGNED, 1), row::MAX_CLUSTER, true)
                          : wide    ? row::plan_row(a.C, 2, 768, row::MAX_CLUSTER, true)
-                                   : row::plan_row(a.C, 4, 512, row::MAX_CLUSTER, true);
+                                   : row::plan_row(a.C, 4, block_limit(row::ALIGNED, 4), row::MAX_CLUSTER, true);
   if (r.units == 0 || a.N > 0x7fffffff / r.cluster) return launch_long();
   const dim3 block(r.threads, r.rows_per_block);
   const unsigned grid = unsigned((a.N + r.rows_per_block - 1) / r.rows_per_block) * r.cluster;

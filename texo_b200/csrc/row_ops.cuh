@@ -64,12 +64,45 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {  // 16-byte 
   for (int i = 0; i < int(sizeof(Raw8<T>) / 16); ++i) __stcs(reinterpret_cast<uint4*>(p) + i, s[i]);
 }
 
-// q = rint(v * inverse) for |v * inverse| < 128: adding this (1.5 * 2^23) rounds to the nearest
-// integer, which is then the sum's low byte (a conversion instruction runs at an eighth of the
-// rate).  inverse 0 stands for a row whose q is zero whatever v is.
+// The per-token quantiser: scale = max(amax, 2^-100) / 127, q = rint(y / scale), both quotients
+// rounded to FP32 first: values half way between two multiples of the scale are common where y
+// has few bits, and a product with a rounded 127 / amax would take them off the tie.
+// The floor keeps scale and reciprocal finite and non-zero for every row (a row of zeros gets
+// q = 0).  A row that holds a NaN or an infinity has no scale that stands for it: its scale is
+// NaN and its q all zero, so that whatever the row is multiplied into shows it.
+constexpr float MIN_TOP = 0x1p-100f;
+struct TokenScale {
+  float scale;
+  float hi, lo;  // 1 / scale in two terms; hi = 0: q is zero whatever y is
+};
+// Quotients by multiplication: scale with a reciprocal and corrections by exact residuals, y / scale
+// (below) with a reciprocal of 48 bits, which rounds like the quotient but for one in 2^23.  A
+// few instructions that every thread can afford, where IEEE divisions take an eighth of a short
+// row's time.
+__device__ __forceinline__ TokenScale token_scale(float amax) {
+  TokenScale s;
+  if (__float_as_uint(amax) >= 0x7f800000u) {
+    s.scale = __int_as_float(0x7fffffff);
+    s.hi = s.lo = 0.f;
+    return s;
+  }
+  const float top = fmaxf(amax, MIN_TOP);
+  constexpr float BY_127 = 1.f / 127.f;
+  float q = __fmul_rn(top, BY_127);
+  q = __fmaf_rn(__fmaf_rn(-127.f, q, top), BY_127, q);
+  s.scale = __fmaf_rn(__fmaf_rn(-127.f, q, top), BY_127, q);
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(s.scale));
+  s.hi = __fmaf_rn(__fmaf_rn(-s.scale, r, 1.f), r, r);
+  s.lo = __fmul_rn(__fmaf_rn(-s.scale, s.hi, 1.f), s.hi);
+  return s;
+}
+// Adding this (1.5 * 2^23) to |t| < 2^22 rounds t to the nearest integer, whose low byte is then the
+// sum's (a conversion instruction runs at an eighth of the rate).
 constexpr float ROUND_TO_INTEGER = 12582912.f;
-__device__ __forceinline__ int8_t quantise(float v, float inverse) {
-  return inverse == 0.f ? int8_t(0) : int8_t(uint8_t(__float_as_uint(__fmaf_rn(v, inverse, ROUND_TO_INTEGER))));
+__device__ __forceinline__ int8_t quantise(float v, const TokenScale& s) {
+  const float quotient = __fmaf_rn(v, s.hi, __fmul_rn(v, s.lo));
+  return s.hi == 0.f ? int8_t(0) : int8_t(uint8_t(__float_as_uint(__fadd_rn(quotient, ROUND_TO_INTEGER))));
 }
 
 // Packed FP32 arithmetic, two values an instruction (each rounded like the scalar one): these
@@ -166,13 +199,15 @@ struct Spread {
   }
 
   // The same for v quantised (ALIGNED: rows start at 8-byte boundaries).
-  __device__ __forceinline__ void store_quantised(int8_t* row, int i, const float (&v)[8], float inverse) const {
+  __device__ __forceinline__ void store_quantised(int8_t* row, int i, const float (&v)[8], const TokenScale& scale) const {
     uint32_t r[8] = {};
-    if (inverse != 0.f) {
-      float sum[8];
-      fma8(sum, v, inverse, float(ROUND_TO_INTEGER));
+    if (scale.hi != 0.f) {
+      float t[8];
+      mul8(t, v, scale.lo);
+      fma8(t, v, scale.hi, t);
+      fma8(t, t, 1.f, float(ROUND_TO_INTEGER));
 #pragma unroll
-      for (int j = 0; j < 8; ++j) r[j] = __float_as_uint(sum[j]);
+      for (int j = 0; j < 8; ++j) r[j] = __float_as_uint(t[j]);
     }
     if (at(i, 0) >= C) return;
     const uint2 q = make_uint2(
@@ -326,27 +361,6 @@ __device__ __forceinline__ float cluster_max(float v, unsigned* scratch, int t, 
   unsigned bits = 0;
   for (int b = 0; b < blocks; ++b) bits = max(bits, maxima[b]);
   return __uint_as_float(bits);
-}
-
-// The per-token quantiser: scale = max(amax, 2^-100) / 127, q = rint(y * (127 / max(amax, 2^-100))),
-// the product unrounded.
-// The floor keeps both quotients finite and non-zero for every row (a row of zeros gets q = 0).
-// A row that holds a NaN or an infinity has no scale that stands for it: its scale is NaN and
-// its q all zero, so that whatever the row is multiplied into shows it.
-constexpr float MIN_TOP = 0x1p-100f;
-__device__ __forceinline__ bool finite(float amax) { return __float_as_uint(amax) < 0x7f800000u; }
-__device__ __forceinline__ float token_scale(float amax) {
-  return finite(amax) ? __fdiv_rn(fmaxf(amax, MIN_TOP), 127.f) : __int_as_float(0x7fffffff);
-}
-// 127 / top, 0 for a row that is not finite.  An approximate reciprocal and one Newton step with an
-// exact residual: within 0.51 units in the last place, in four instructions that every thread
-// can afford (the IEEE division takes an eighth of a short row's instructions).
-__device__ __forceinline__ float token_inverse(float amax) {
-  const float top = fmaxf(amax, MIN_TOP);
-  float r;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(top));
-  const float q = __fmul_rn(127.f, r);
-  return finite(amax) ? __fmaf_rn(__fmaf_rn(-top, q, 127.f), r, q) : 0.f;
 }
 
 // ------------------------------------------------------------------- host side
