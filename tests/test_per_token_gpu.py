@@ -510,6 +510,29 @@ def test_producers_write_their_outputs_alone(ops, shape, shift):
             assert bool((base[:64 + shift] == 77).all()) and bool((base[64 + shift + N * (C // 2):] == 77).all())
 
 
+@pytest.mark.parametrize("C", [8192, 8191])
+def test_producers_past_32_bit_offsets(ops, C):
+    """Rows whose elements lie beyond the 2^31st."""
+    N = 270000
+    x = torch.empty((N, C), dtype=torch.bfloat16, device="cuda").uniform_(-2, 2, generator=generator(1))
+    rows = torch.tensor([0, 1, 131072, 262143, 262144, N - 2, N - 1], device="cuda")
+    w = torch.ones(C, device="cuda", dtype=torch.bfloat16)
+
+    def check(q, s, z):
+        part = x[rows]
+        q1, s1, z1 = ops.block_norm_quant_per_token(part, part, w, 1e-5)
+        y64, dy, z64, dz = norm_expected(part, part, w, None, None, 1e-5, 1.0)
+        check_quantised(q, s, y64, dy)
+        assert_within(z, z64, dz + half_step(z64, torch.bfloat16) * 1.01)
+        assert torch.equal(z, z1)
+
+    q, s = ops.quant_per_token(x)
+    assert N * C > 2 ** 31
+    check_quantised(q[rows], s[rows], x[rows].double(), torch.zeros((len(rows), C), dtype=torch.float64, device="cuda"))
+    q, s, z = ops.block_norm_quant_per_token(x, x, w, 1e-5)
+    check(q[rows], s[rows], z[rows])
+
+
 def test_swiglu_of_far_gates(ops):
     gate = torch.tensor([-1e4, -200.0, -100.0, -88.0, -87.0, 88.0, 200.0, 1e4], device="cuda")
     up = torch.full_like(gate, 2.0)

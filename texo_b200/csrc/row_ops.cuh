@@ -153,11 +153,9 @@ struct Spread {
   int t, threads, C;
   __device__ __forceinline__ int at(int i, int j) const { return (i * threads + t) * 8 + j; }
 
-  // Whether group i of every thread lies within the row.
-  __device__ __forceinline__ bool full(int i) const { return (i + 1) * threads * 8 <= C; }
   // Makes the values past the row's end zero.
   __device__ __forceinline__ void mask(int i, float (&v)[8]) const {
-    if (full(i)) return;
+    if (at(i, 8) <= C) return;
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       if (at(i, j) >= C) v[j] = 0.f;
