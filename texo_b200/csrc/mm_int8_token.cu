@@ -135,9 +135,10 @@ __global__ void __launch_bounds__(G_THREADS)
 //
 // A tile (256 columns x R rows) is worked on by a cluster of c CTAs, each on its own part of K.
 // There is no workspace: once all of them are through, every CTA pushes its int32 partials
-// straight into the shared memory (the ring, idle by then) of the CTA that finishes the row, row
-// r going to CTA r % c; an mbarrier there counts the pushes, and the owner adds the c copies,
-// scales and stores.  Integer sums, so the split changes no bit, and nothing is shared between
+// straight into the shared memory (the ring, idle by then) of the CTA that finishes the rows, four
+// rows at a time (a 16-byte store per lane; 4-byte ones took 5.8 of 47 us at 128 x 8192 x
+// 28672), quad g going to CTA g % c; an mbarrier there counts the pushes, and the owner adds the c
+// copies, scales and stores.  Integer sums, so the split changes no bit, and nothing is shared between
 // calls: any streams, any graphs.  With c = 1 the lanes, each one output column, scale and store
 // from registers while the ring fills for the next tile.
 //
@@ -175,12 +176,12 @@ __host__ __device__ constexpr int s_ring_bytes(int R, bool gather) {
 __host__ __device__ constexpr int s_smem_bytes(int R, bool gather) {
   return s_ring_bytes(R, gather) + 1024 /*alignment*/ + 256 /*barriers*/;
 }
-// Rows of a tile that one CTA of the cluster finishes, and the room that their partials take.
-__host__ __device__ constexpr int s_slots(int R, int c) { return (R + c - 1) / c; }
-__host__ __device__ constexpr int s_push_bytes(int R, int c) { return c * s_slots(R, c) * S_TILE_N * 4; }
-constexpr int SMEM_LIMIT = 232448;
+// Row quads of a tile that one CTA of the cluster finishes, and the room that their partials take.
+__host__ __device__ constexpr int s_slots(int R, int c) { return (R / 4 + c - 1) / c; }
+__host__ __device__ constexpr int s_push_bytes(int R, int c) { return c * s_slots(R, c) * S_TILE_N * 16; }
+constexpr int SMEM_LIMIT = 232448, S_SMEM_LIMIT = SMEM_LIMIT - S_EPI_WARPS * 128 * 4 /*row scales*/;
 __host__ __device__ constexpr bool s_fits(int R, bool gather) {
-  return s_smem_bytes(R, gather) <= SMEM_LIMIT && s_push_bytes(R, 7) <= s_ring_bytes(R, gather) &&
+  return s_smem_bytes(R, gather) <= S_SMEM_LIMIT && s_push_bytes(R, 7) <= s_ring_bytes(R, gather) &&
          s_push_bytes(R, 6) <= s_ring_bytes(R, gather) && s_push_bytes(R, 5) <= s_ring_bytes(R, gather) &&
          s_push_bytes(R, 3) <= s_ring_bytes(R, gather) && s_push_bytes(R, 8) <= s_ring_bytes(R, gather);
 }
@@ -203,8 +204,10 @@ struct StreamBarriers {
 };
 static_assert(sizeof(StreamBarriers) <= 256, "StreamBarriers outgrew its shared-memory reserve");
 
-__device__ __forceinline__ void store_cluster_u32(uint32_t cluster_addr, uint32_t v) {
-  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
+__device__ __forceinline__ void store_cluster_quad(uint32_t cluster_addr, uint32_t a, uint32_t b, uint32_t c,
+                                                   uint32_t d) {
+  asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_addr), "r"(a), "r"(b), "r"(c), "r"(d)
+               : "memory");
 }
 
 // After a wait gave up: gives the loads in flight a tenth of a second to land before the CTA's
@@ -374,7 +377,6 @@ __device__ __forceinline__ void shift_rows(uint32_t to, uint32_t granules, const
 struct StreamShape {
   int M, N, K;
   int R, cluster, m_tiles, tiles;
-  int vector_out;  // rows of the output start at 16-byte boundaries
 };
 
 template <typename Y, bool GATHER>
@@ -383,6 +385,7 @@ __global__ void __launch_bounds__(GATHER ? S_GATHER_THREADS : S_THREADS, 1)
                   const int8_t* __restrict__ A, const int8_t* __restrict__ B, Y* __restrict__ out, Scales s,
                   StreamShape p, int* status) {
   extern __shared__ uint8_t smem_raw[];
+  __shared__ float row_scales[S_EPI_WARPS][128];  // scale_A of the tile's rows, a copy for each warp
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   grid_dependency_trigger();
   const int R = p.R, c = p.cluster;
@@ -567,6 +570,10 @@ __global__ void __launch_bounds__(GATHER ? S_GATHER_THREADS : S_THREADS, 1)
     // ---------------------------------------------------------------- epilogue
     const int ew = warp - 2, quarter = warp % 4, half = ew / 4;
     const int column = half * 128 + quarter * 32 + lane;  // of the tile
+    // The finished values are dealt out by columns: warp ew has 32 of each row (c = 1: those that its
+    // lanes read from tensor memory).
+    const int own_column = c == 1 ? column : ew * 32 + lane;
+    float* scales_a = row_scales[ew];
     int buf = 0;
     uint32_t buf_phase = 0, tile_phase = 0;
     bool ok = true;
@@ -574,26 +581,27 @@ __global__ void __launch_bounds__(GATHER ? S_GATHER_THREADS : S_THREADS, 1)
     for (int tile = first_tile; tile < p.tiles && ok; tile += tile_step) {
       const int n0 = tile / p.m_tiles * S_TILE_N, m0 = tile % p.m_tiles * R;
       const int rows = min(R, p.M - m0);
+      // the scales travel while the accumulator fills
+      const int n = n0 + own_column;
+      const bool in = n < p.N;
+      const float sb = in ? __ldg(s.b + n) : 0.f, bias = in && s.bias ? __ldg(s.bias + n) : 0.f;
+      __syncwarp();
+      for (int r = lane; r < rows; r += 32) scales_a[r] = __ldg(s.a + m0 + r);
+      __syncwarp();
+      Y* column_out = out + size_t(m0) * p.N + n;
       ok = warp_wait(&bars->acc_full[buf], buf_phase, abort_flag, status, STATUS_TIMEOUT_TMEM_FULL);
       if (!ok) break;
       tc_fence_after_sync();
       const uint32_t acc = tmem_base + (buf * 2 + half) * R + (uint32_t(quarter * 32) << 16);
       if (c == 1) {
-        const int n = n0 + column;
-        const bool in = n < p.N;
-        const float sb = in ? __ldg(s.b + n) : 0.f, bias = in && s.bias ? __ldg(s.bias + n) : 0.f;
-        Y* column_out = out + size_t(m0) * p.N + n;
         for (int r0 = 0; r0 < rows; r0 += 16) {
           uint32_t v[16];
           tmem_ld_32x16(acc + r0, v);
-          const int m = min(m0 + r0 + lane % 16, p.M - 1);
-          const float sa_lane = __ldg(s.a + m);
           tmem_ld_wait();
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const float sa = __shfl_sync(0xffffffffu, sa_lane, r);
             if (in && r0 + r < rows)
-              column_out[size_t(r0 + r) * p.N] = row::from_float<Y>(scaled(float(int(v[r])), sa, sb, bias));
+              column_out[size_t(r0 + r) * p.N] = row::from_float<Y>(scaled(float(int(v[r])), scales_a[r0 + r], sb, bias));
           }
         }
         tc_fence_before_sync();
@@ -605,7 +613,7 @@ __global__ void __launch_bounds__(GATHER ? S_GATHER_THREADS : S_THREADS, 1)
         ok = warp_wait_cluster(&bars->ring_idle, tile_phase, abort_flag, status, STATUS_TIMEOUT_FLAG);
         if (!ok) break;
         const int slots = s_slots(R, c);
-        const uint32_t to = push + uint32_t((rank * slots * S_TILE_N + column) * 4);
+        const uint32_t to = push + uint32_t((rank * slots * S_TILE_N + column) * 16);
         int owner = 0;
         uint32_t slot_bytes = 0;
         for (int r0 = 0; r0 < rows; r0 += 16) {
@@ -613,12 +621,12 @@ __global__ void __launch_bounds__(GATHER ? S_GATHER_THREADS : S_THREADS, 1)
           tmem_ld_32x16(acc + r0, v);
           tmem_ld_wait();
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
+          for (int r = 0; r < 16; r += 4) {
             if (r0 + r < rows) {
-              store_cluster_u32(map_to_cta(to + slot_bytes, owner), v[r]);
+              store_cluster_quad(map_to_cta(to + slot_bytes, owner), v[r], v[r + 1], v[r + 2], v[r + 3]);
               if (++owner == c) {
                 owner = 0;
-                slot_bytes += S_TILE_N * 4;
+                slot_bytes += S_TILE_N * 16;
               }
             }
           }
@@ -629,39 +637,17 @@ __global__ void __launch_bounds__(GATHER ? S_GATHER_THREADS : S_THREADS, 1)
         if (lane < c) mbar_arrive_cluster(map_to_cta(smem_u32(&bars->pushed), lane));
         ok = warp_wait_cluster(&bars->pushed, tile_phase, abort_flag, status, STATUS_TIMEOUT_FLAG);
         if (!ok) break;
-        for (int slot = ew; slot * c + rank < rows; slot += S_EPI_WARPS) {
-          const int m = m0 + slot * c + rank;
-          const uint32_t first = push + slot * S_TILE_N * 4;
-          const float sa = __ldg(s.a + m);
-          Y* row_out = out + size_t(m) * p.N + n0;
-          if (p.vector_out && n0 + lane * 8 + 8 <= p.N) {
-            int total[8] = {};
-            for (int copy = 0; copy < c; ++copy) {
-              const uint32_t w = first + (copy * slots * S_TILE_N + lane * 8) * 4;
-              const int4 lo = lds128(w), hi = lds128(w + 16);
-              total[0] += lo.x, total[1] += lo.y, total[2] += lo.z, total[3] += lo.w;
-              total[4] += hi.x, total[5] += hi.y, total[6] += hi.z, total[7] += hi.w;
-            }
-            float y[8];
+        for (int slot = 0; (slot * c + rank) * 4 < rows; ++slot) {
+          const int r0 = (slot * c + rank) * 4;
+          int total[4] = {};
+          for (int copy = 0; copy < c; ++copy) {
+            const int4 x = lds128(push + uint32_t(((copy * slots + slot) * S_TILE_N + own_column) * 16));
+            total[0] += x.x, total[1] += x.y, total[2] += x.z, total[3] += x.w;
+          }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const int n = n0 + lane * 8 + e;
-              y[e] = scaled(float(total[e]), sa, __ldg(s.b + n), s.bias ? __ldg(s.bias + n) : 0.f);
-            }
-            row::store8(row_out + lane * 8, y);
-          } else if (!p.vector_out) {
-            int total[8] = {};
-            for (int copy = 0; copy < c; ++copy) {
-#pragma unroll
-              for (int j = 0; j < 8; ++j) total[j] += int(lds32(first + (copy * slots * S_TILE_N + j * 32 + lane) * 4));
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const int n = n0 + j * 32 + lane;
-              if (n < p.N)
-                row_out[j * 32 + lane] = row::from_float<Y>(
-                    scaled(float(total[j]), sa, __ldg(s.b + n), s.bias ? __ldg(s.bias + n) : 0.f));
-            }
+          for (int e = 0; e < 4; ++e) {
+            if (in && r0 + e < rows)
+              column_out[size_t(r0 + e) * p.N] = row::from_float<Y>(scaled(float(total[e]), scales_a[r0 + e], sb, bias));
           }
         }
         fence_proxy_async_smem();  // these accesses come before the loads that fill the ring again
@@ -1100,8 +1086,8 @@ struct DeviceSetup {
 static DeviceSetup setups[MAX_DEVICES];
 template <typename Y>
 static void configure_kernels() {
-  cudaFuncSetAttribute(stream_kernel<Y, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
-  cudaFuncSetAttribute(stream_kernel<Y, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
+  cudaFuncSetAttribute(stream_kernel<Y, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, S_SMEM_LIMIT);
+  cudaFuncSetAttribute(stream_kernel<Y, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, S_SMEM_LIMIT);
   cudaFuncSetAttribute(pair_kernel<Y, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, P_SMEM_BYTES);
   cudaFuncSetAttribute(pair_kernel<Y, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, P_SMEM_BYTES);
 }
@@ -1127,14 +1113,16 @@ static DeviceSetup& device_setup(DeviceCtx& ctx) {
 
 // The choice between the paths, and of R and c, is by estimated time in microseconds.  The constants
 // are fits to measurements on B200 (kernels back to back, operands from HBM):
-//   stream, per k block of 128: 0.42 + 0.0009 R, or its 32 KiB of B at 6.2 TB/s over all CTAs
-//   gather, per k block: 1.3 up to R = 32, then 1.8 (64) and 2.8 (128): shared-memory bandwidth
-//   either, per round of tiles: 0.3 (c = 1) or 2, per call: 2.2 or 2.7, and 0.045 R for the drain
-//     (0.065 R where rows of Y are not multiples of eight)
+//   stream, per k block of 128: 0.44 + 0.0009 R, or its 32 KiB of B at 7.1 TB/s over all CTAs
+//   gather, per k block: 1.4 up to R = 32, then 1.7 (64) and 2.6 (128): shared-memory bandwidth;
+//     1.5 more per call
+//   either, per round of tiles: 0.3 (c = 1) or 3, per call: 2.2 or 1.9 + 0.2 c, and 0.035 R for
+//     the drain
 //   pair, per k block 0.33 (0.42 once all SMs run: power), per call 7, per round of tiles 1
-//   padding: 2.5 and twice the operand's bytes at 5 TB/s
+//   padding: 1.5 and twice the operand's bytes at 6 TB/s
 // E.g. 512 x 512 x 1024: streaming at R = 16, 32, 128 6.5, 7.3, 12 us, pairs 10.7; 256 x 4096 x
-// 4096: 17.0 against 19.7; 1024 x 4096 x 4096: 25 against 19.9.
+// 4096: 15.7 against 19.6; 1024 x 4096 x 4096: 25 against 19.9.  Over 136 aligned sizes the choice costs 1%
+// more than the best one, 18% at worst (202 x 176 x 11408: 14.3 for 12.1).
 struct StreamPlan {
   int R = 0, cluster = 0, clusters = 0, m_tiles = 0, tiles = 0;
   double us = 1e30;
@@ -1151,10 +1139,10 @@ static StreamPlan plan_stream(const DeviceSetup& d, bool gather, int M, int N, i
       if (held <= 0) continue;
       const int clusters = int(std::min<long long>(tiles, held));
       const double rounds = double((tiles + clusters - 1) / clusters);
-      const double block = gather ? (R <= 32 ? 1.3 : R == 64 ? 1.8 : 2.8)
-                                  : std::max(0.42 + 0.0009 * R, 32768.0 * clusters * c / double(m_tiles) / 6.2e6);
-      const double us = rounds * ((num_kb + c - 1) / c * block + (c > 1 ? 2 : 0.3)) + (c > 1 ? 2.7 : 2.2) +
-                        (N % 8 == 0 ? 0.045 : 0.065) * R;
+      const double block = gather ? (R <= 32 ? 1.4 : R == 64 ? 1.7 : 2.6)
+                                  : std::max(0.44 + 0.0009 * R, 32768.0 * clusters * c / double(m_tiles) / 7.1e6);
+      const double us = rounds * ((num_kb + c - 1) / c * block + (c > 1 ? 3 : 0.3)) + (c > 1 ? 1.9 + 0.2 * c : 2.2) +
+                        0.035 * R + (gather ? 1.5 : 0);
       if (us < best.us) best = {R, c, clusters, int(m_tiles), int(tiles), us};
     }
     if (M <= R) break;  // a larger R only pads
@@ -1179,7 +1167,7 @@ static Route choose_route(const DeviceSetup& d, int M, int N, int K, bool a_ok, 
   if (K <= 0 || K >= (1 << 17) || force == PATH_GENERIC) return best;
   const long long pad = pad_bytes(M, N, K, !a_ok, !b_ok);
   if (pad <= workspace && force != PATH_STREAM_GATHER) {
-    const double pad_us = pad ? 2.5 + 2.0 * double(pad) / 5e6 : 0;
+    const double pad_us = pad ? 1.5 + 2.0 * double(pad) / 6e6 : 0;
     if (force != PATH_PAIR) {
       const StreamPlan plan = plan_stream(d, false, M, N, K);
       if (plan.cluster > 0) best = {PATH_STREAM, !a_ok, !b_ok, plan, plan.us + pad_us};
@@ -1213,8 +1201,7 @@ static bool launch_stream(DeviceCtx& ctx, const StreamPlan& plan, const Operand&
                   !make_tensor_map_2d(&map_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, A.p, M, K, A.pitch, plan.R, S_BK,
                                       CU_TENSOR_MAP_SWIZZLE_128B)))
     return false;
-  const StreamShape p = {M, N, K, plan.R, plan.cluster, plan.m_tiles, plan.tiles,
-                         N % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0};
+  const StreamShape p = {M, N, K, plan.R, plan.cluster, plan.m_tiles, plan.tiles};
   return launch_on_stream(stream_kernel<Y, GATHER>, plan.clusters * plan.cluster,
                          GATHER ? S_GATHER_THREADS : S_THREADS, s_smem_bytes(plan.R, GATHER), plan.cluster, stream,
                          map_b, map_a, A.p, B.p, out, s, p, ctx.status);
