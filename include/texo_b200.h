@@ -22,7 +22,7 @@
  * (The dynamic-quantisation operators at the end of this file take the stream as an argument,
  * return a code and own no scratch memory.)
  * Scratch memory is owned by the library (per device, grow-only, never freed).  Calls are
- * not thread-safe.
+ * not thread-safe, but for the dynamic-quantisation operators.
  */
 #ifndef TEXO_B200_H
 #define TEXO_B200_H
@@ -298,11 +298,12 @@ double texo_int8_feed_rate_tbs(const void* A, const void* B, int M, int N, int K
  *
  * `stream` is a cudaStream_t; null is the legacy default stream.  The work is issued on it
  * asynchronously; the library owns no scratch memory for it, so calls on different streams may
- * overlap, and calls may be captured into a graph once the same call has been made outside of
- * capture (the product's first call on a device sets the device up and refuses to do so while
- * capturing).  Returns 0, -1 bad arguments, -2 a size within a few thousand of 2^31 or beyond, -3
- * a launch was refused, -4 first product on this device while capturing.  A bounded device-side
- * wait that gave up inside a product shows in texo_mm_int8_status().  Element types: */
+ * overlap and several threads may make them, and calls may be captured into a graph once the same
+ * call has been made outside of capture (the product's first call on a device sets the device up
+ * and refuses to do so while capturing).  Returns 0, -1 bad arguments, -2 a size within a few
+ * thousand of 2^31 or beyond, -3 a launch was refused, -4 first product on this device while
+ * capturing.  A bounded device-side wait that gave up inside a product shows in
+ * texo_mm_int8_status().  Element types: */
 #define TEXO_F16 0
 #define TEXO_BF16 1
 #define TEXO_F32 2

@@ -614,6 +614,30 @@ def test_two_streams_at_once(ops):
             assert all(torch.equal(a, b) for a, b in zip(want, got))
 
 
+def test_several_threads_at_once(ops):
+    # more operand pairs than the library keeps tensor maps of
+    from concurrent.futures import ThreadPoolExecutor
+
+    threads, pairs = 4, 12
+    sets = [[mm_inputs(8 + 16 * i, 128 + 16 * i, 256 + 32 * t, 100 * t + i) for i in range(pairs)] for t in range(threads)]
+    torch.cuda.synchronize()
+
+    def work(mine):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            results = [ops.mm_int8_per_token(*mine[k % pairs], out_dtype=torch.float32) for k in range(10 * pairs)]
+        stream.synchronize()
+        return results
+
+    with ThreadPoolExecutor(threads) as pool:
+        everything = list(pool.map(work, sets))
+    for mine, results in zip(sets, everything):
+        for i, operands in enumerate(mine):
+            want = ops.mm_int8_per_token(*operands, out_dtype=torch.float32)
+            for got in results[i::pairs]:
+                assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("n", [1, 16, 200])
 def test_captured_and_replayed(ops, n):
     x, residual, w = mlp_setup(n, 512, 1024)

@@ -6,11 +6,15 @@
 // :9-12 of frezcirno/Texo): work is issued on the legacy default stream of the current
 // device, asynchronously, and the scratch is callee-owned, process-static and never freed.
 // Unlike the reference, the state is kept per device, so one process may drive several GPUs
-// (one after another; calls are still not thread-safe).
+// (one after another; calls of those operators are still not thread-safe).  What the operators on
+// the caller's stream share with them - device set-up, the tensor-map cache, the launch counter -
+// may be used from several threads.
 #pragma once
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
 #include <cstdio>
+#include <mutex>
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -19,7 +23,7 @@ namespace texo {
 constexpr int MAX_DEVICES = 64;
 
 struct DeviceCtx {
-  bool ready = false;
+  std::atomic<bool> ready{false};
   int device = -1;
   int sm_count = 0;
   int cc_major = 0;
@@ -55,9 +59,17 @@ inline DeviceCtx& device_ctx_entry(int& device) {
   return table[device];
 }
 
+// Held while a device is set up.
+inline std::mutex& setup_mutex() {
+  static std::mutex m;
+  return m;
+}
+
 inline DeviceCtx& device_ctx() {
   int device;
   DeviceCtx& ctx = device_ctx_entry(device);
+  if (ctx.ready) return ctx;
+  std::lock_guard<std::mutex> lock(setup_mutex());
   if (!ctx.ready) {
     ctx.device = device;
     cudaDeviceGetAttribute(&ctx.sm_count, cudaDevAttrMultiProcessorCount, device);
@@ -181,8 +193,8 @@ inline cudaError_t launch_overlapping_predecessor(void (*kernel)(Params...), dim
 
 // ------------------------------------------------------------ instrumentation
 // Cumulative number of kernels this library has launched (all devices).
-inline long long& launch_counter() {
-  static long long count = 0;
+inline std::atomic<long long>& launch_counter() {
+  static std::atomic<long long> count{0};
   return count;
 }
 
@@ -254,19 +266,16 @@ using TensorMapEncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint
                                        CUtensorMapFloatOOBfill);
 
 inline TensorMapEncodeFn tensor_map_encoder() {
-  static TensorMapEncodeFn fn = nullptr;
-  static bool tried = false;
-  if (!tried) {
-    tried = true;
+  static const TensorMapEncodeFn fn = [] {
     void* entry = nullptr;
     cudaDriverEntryPointQueryResult result;
     if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &entry, cudaEnableDefault, &result) ==
             cudaSuccess &&
         result == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<TensorMapEncodeFn>(entry);
-    else
-      cudaGetLastError();
-  }
+      return reinterpret_cast<TensorMapEncodeFn>(entry);
+    cudaGetLastError();
+    return TensorMapEncodeFn(nullptr);
+  }();
   return fn;
 }
 
@@ -291,6 +300,7 @@ struct TensorMapKey {
 };
 constexpr int TENSOR_MAP_CACHE_SLOTS = 32;
 struct TensorMapCache {
+  std::mutex mutex;
   TensorMapKey key[TENSOR_MAP_CACHE_SLOTS];
   CUtensorMap map[TENSOR_MAP_CACHE_SLOTS];
   int used = 0, next = 0;
@@ -306,6 +316,7 @@ inline bool make_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType type, size_
                                uint64_t row_pitch_bytes, uint32_t box_rows, uint32_t box_cols,
                                CUtensorMapSwizzle swizzle) {
   TensorMapCache& cache = tensor_map_cache();
+  std::lock_guard<std::mutex> lock(cache.mutex);
   const TensorMapKey key = {base, rows, cols, row_pitch_bytes, box_rows, box_cols, int(type), int(swizzle)};
   for (int i = 0; i < cache.used; ++i) {
     if (cache.key[i] == key) {

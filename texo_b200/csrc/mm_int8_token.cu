@@ -1029,12 +1029,12 @@ __global__ void __launch_bounds__(PAD_THREADS) pad_kernel(const Pad a, const Pad
 
 // ------------------------------------------------------------------ dispatch
 enum Path { PATH_AUTO = 0, PATH_GENERIC = 1, PATH_STREAM = 2, PATH_STREAM_GATHER = 3, PATH_PAIR = 4 };
-inline int& forced_path() {
-  static int path = 0;
+inline std::atomic<int>& forced_path() {
+  static std::atomic<int> path{0};
   return path;
 }
-inline int& last_path() {
-  static int path = 0;
+inline std::atomic<int>& last_path() {
+  static std::atomic<int> path{0};
   return path;
 }
 
@@ -1079,7 +1079,7 @@ static int max_clusters(Kernel kernel, int threads, int smem_bytes, int cluster)
 
 constexpr int R_CHOICES[4] = {16, 32, 64, 128};
 struct DeviceSetup {
-  bool ready = false;
+  std::atomic<bool> ready{false};
   int clusters[2][4][S_MAX_CLUSTER + 1] = {};  // [gather][R][c]
   int pairs = 0;
 };
@@ -1093,6 +1093,8 @@ static void configure_kernels() {
 }
 static DeviceSetup& device_setup(DeviceCtx& ctx) {
   DeviceSetup& d = setups[ctx.device];
+  if (d.ready) return d;
+  std::lock_guard<std::mutex> lock(setup_mutex());
   if (!d.ready) {
     configure_kernels<__half>();
     configure_kernels<__nv_bfloat16>();

@@ -33,7 +33,7 @@ struct Args {
 // gate and up are never multiplied first: their product can overflow where the result does not.
 // The exponential is that of __expf (a product with log2 e, then ex2.approx), the reciprocal
 // rcp.approx; both flush subnormals, which saves the scaling around them: a denominator beyond
-// 2^126 (gate < -87) gives 0 where the value is below 2^-118.
+// 2^126 (gate < -87) makes silu(gate) 0, less than 2^-118 away from what it is.
 __device__ __forceinline__ float swiglu(float gate, float up) {
   float e, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmul_rn(gate, -1.44269504f)));
