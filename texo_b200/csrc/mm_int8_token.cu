@@ -1115,10 +1115,10 @@ static DeviceSetup& device_setup(DeviceCtx& ctx) {
 
 // The choice between the paths, and of R and c, is by estimated time in microseconds.  The constants
 // are fits to measurements on B200 (kernels back to back, operands from HBM):
-//   stream, per k block of 128: 0.44 + 0.0009 R, or its 32 KiB of B at 7.1 TB/s over all CTAs
+//   stream, per k block of 128: 0.42 + 0.0009 R, or its 32 KiB of B at 7.1 TB/s over all CTAs
 //   gather, per k block: 1.4 up to R = 32, then 1.7 (64) and 2.6 (128): shared-memory bandwidth;
 //     1.5 more per call
-//   either, per round of tiles: 0.3 (c = 1) or 3, per call: 2.2 or 1.9 + 0.2 c, and 0.035 R for
+//   either, per round of tiles: 0.3 (c = 1) or 2.5, per call: 2.2 or 2 + 0.15 c, and 0.035 R for
 //     the drain
 //   pair, per k block 0.33 (0.42 once all SMs run: power), per call 7, per round of tiles 1
 //   padding: 1.5 and twice the operand's bytes at 6 TB/s
@@ -1142,8 +1142,8 @@ static StreamPlan plan_stream(const DeviceSetup& d, bool gather, int M, int N, i
       const int clusters = int(std::min<long long>(tiles, held));
       const double rounds = double((tiles + clusters - 1) / clusters);
       const double block = gather ? (R <= 32 ? 1.4 : R == 64 ? 1.7 : 2.6)
-                                  : std::max(0.44 + 0.0009 * R, 32768.0 * clusters * c / double(m_tiles) / 7.1e6);
-      const double us = rounds * ((num_kb + c - 1) / c * block + (c > 1 ? 3 : 0.3)) + (c > 1 ? 1.9 + 0.2 * c : 2.2) +
+                                  : std::max(0.42 + 0.0009 * R, 32768.0 * clusters * c / double(m_tiles) / 7.1e6);
+      const double us = rounds * ((num_kb + c - 1) / c * block + (c > 1 ? 2.5 : 0.3)) + (c > 1 ? 2 + 0.15 * c : 2.2) +
                         0.035 * R + (gather ? 1.5 : 0);
       if (us < best.us) best = {R, c, clusters, int(m_tiles), int(tiles), us};
     }
