@@ -113,8 +113,8 @@ __global__ void __launch_bounds__(block_limit(L, UNITS), blocks_per_sm(L, UNITS)
   __shared__ unsigned scratch[row::MAX_WARPS], maxima[row::MAX_CLUSTER];
   grid_dependency_trigger();
   row::cluster_started(blocks);
-  const int part = int(blockIdx.x) % blocks;  // of the row
-  const long long n = (long long)(blockIdx.x / blocks) * blockDim.y + threadIdx.y;
+  const int part = int(cluster_ctarank());  // of the row
+  const long long n = (long long)cluster_id() * blockDim.y + threadIdx.y;
   if (n >= a.N) return;  // only blocks of one-warp rows reach past N; they meet at no barrier
   const int t = threadIdx.x, threads = blockDim.x;
   const row::Spread<L> s = {part * threads + t, blocks * threads, a.C};
