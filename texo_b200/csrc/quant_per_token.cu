@@ -41,13 +41,23 @@ __device__ __forceinline__ float swiglu(float gate, float up) {
   return gate * r * up;
 }
 
+// The same of eight, in packed arithmetic (and the same bits).
+__device__ __forceinline__ void swiglu8(const float (&gate)[8], const float (&up)[8], float (&y)[8]) {
+  float t[8];
+  row::mul8(t, gate, -1.44269504f);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(t[j]));
+  row::fma8(t, t, 1.f, 1.f);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(t[j]));
+  row::mul8(t, gate, t);
+  row::mul8(y, t, up);
+}
 // Eight outputs from sixteen interleaved inputs.
 __device__ __forceinline__ void swiglu_pairs(const float (&lo)[8], const float (&hi)[8], float (&y)[8]) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    y[j] = swiglu(lo[2 * j], lo[2 * j + 1]);
-    y[4 + j] = swiglu(hi[2 * j], hi[2 * j + 1]);
-  }
+  const float gate[8] = {lo[0], lo[2], lo[4], lo[6], hi[0], hi[2], hi[4], hi[6]};
+  const float up[8] = {lo[1], lo[3], lo[5], lo[7], hi[1], hi[3], hi[5], hi[7]};
+  swiglu8(gate, up, y);
 }
 
 // Group i of an aligned row in global memory, as y; values past the end are zero.
@@ -59,8 +69,7 @@ __device__ __forceinline__ void load_y(const X* x, const row::Spread<row::ALIGNE
     float g[8], u[8];
     s.template load<true>(x, i, g);
     s.template load<true>(x + s.C, i, u);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = swiglu(g[j], u[j]);
+    swiglu8(g, u, y);
   } else {
     // the sixteen inputs of eight outputs: two groups of a row of 2 C values
     const row::Spread<row::ALIGNED> wide = {0, 1, 2 * s.C};
@@ -90,16 +99,13 @@ __device__ __forceinline__ void read_y(uint32_t first, unsigned offset, uint32_t
     if (FORM == SWIGLU_HALVES) {
       float u[8];
       row::read_staged<X>(second, second_offset, s.at(i, 0), u);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = swiglu(y[j], u[j]);
+      swiglu8(y, u, y);
     }
   }
   s.mask(i, y);  // (what lies past the row's end is arbitrary)
 }
 
-// Threads of a block at most, and such blocks that an SM has to hold for their latencies to overlap:
-// with two groups per thread in 40 registers instead of 32, 4096 x 28672 interleaved pairs took
-// 148 us instead of 131.
+// Threads of a block at most, and such blocks that an SM has to hold for their latencies to overlap.
 __host__ __device__ constexpr int block_limit(row::Layout layout, int units) {
   return layout == row::STAGED || units < 4 ? 1024 : 512;
 }
@@ -196,20 +202,16 @@ static bool launch(const Args& a, cudaStream_t stream) {
     auto rows = [&](auto* kernel) { return row::launch_staged(kernel, unsigned(a.N), dim3(r.threads), room, stream, a, 1); };
     return r.units == 1 ? rows(row_kernel<X, FORM, row::STAGED, 1>) : rows(row_kernel<X, FORM, row::STAGED, 4>);
   }
-  // One group per thread while rows do not fill the GPU.  Once they do: four (8192 x 8192 BF16:
-  // 60 / 41 / 35 us for one / two / four), or two where 16-bit pairs are interleaved, whose groups
-  // are twice as wide (4096 x 11008: 45 / 50 us for two / four).
-  const bool wide = FORM == SWIGLU_INTERLEAVED && sizeof(X) == 2;
+  // One group per thread while rows do not fill the GPU.  Once they do, four: a thread's fixed
+  // work (its place, the reduction, the scale) is spread over more values (8192 x 8192 BF16: 60 /
+  // 41 / 35 us for one / two / four; 4096 x 28672 interleaved pairs: 145 / 120 us for two / four).
   const row::RowPlan r = a.N < 512 ? row::plan_row(a.C, 1, block_limit(row::ALIGNED, 1), row::MAX_CLUSTER, true)
-                         : wide    ? row::plan_row(a.C, 2, 768, row::MAX_CLUSTER, true)
                                    : row::plan_row(a.C, 4, block_limit(row::ALIGNED, 4), row::MAX_CLUSTER, true);
   if (r.units == 0 || a.N > 0x7fffffff / r.cluster) return launch_long();
   const dim3 block(r.threads, r.rows_per_block);
   const unsigned grid = unsigned((a.N + r.rows_per_block - 1) / r.rows_per_block) * r.cluster;
   auto rows = [&](auto* kernel) { return launch_on_stream(kernel, grid, block, 0, r.cluster, stream, a, r.cluster); };
-  return r.units == 1   ? rows(row_kernel<X, FORM, row::ALIGNED, 1>)
-         : r.units == 2 ? rows(row_kernel<X, FORM, row::ALIGNED, 2>)
-                        : rows(row_kernel<X, FORM, row::ALIGNED, 4>);
+  return r.units == 1 ? rows(row_kernel<X, FORM, row::ALIGNED, 1>) : rows(row_kernel<X, FORM, row::ALIGNED, 4>);
 }
 
 template <int FORM>
