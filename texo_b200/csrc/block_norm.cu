@@ -255,10 +255,10 @@ static bool launch(const Args& a, cudaStream_t stream) {
   const bool aligned_rows = a.C % 8 == 0 && aligned(a.x, 16) && aligned(a.residual, 16) && aligned(a.weight, 16) &&
                       aligned(a.post_weight, 16) && (aligned(a.gate, 16) || !a.gate_per_channel) &&
                       aligned(a.z, 16) && (QUANT ? aligned(a.q, 8) : aligned(a.y, 16));
-  // One group per thread is the shortest way through a row, for when rows do not fill the GPU;
-  // two measured best once they do (4096 x 8192 BF16, both norms, gate, quantised: 92 / 59 / 71 us
-  // for one / two / four).
-  const row::RowPlan r = row::plan_row(a.C, a.N < 512 && a.C <= 8192 ? 1 : 2, 1024, 1, aligned_rows);
+  // Both norms, gate, quantised, BF16: 4096 x 8192 92 / 59 / 71 us for one / two / four groups per
+  // thread, 128 x 8191 7.6 / 9.1 for one / two, 300 x 8191 20 / 16.
+  row::RowPlan r = row::plan_row(a.C, 1, 1024, 1, aligned_rows);
+  if (!row::at_once(r, a.N, 1024)) r = row::plan_row(a.C, 2, 1024, 1, aligned_rows);
   if (r.units == 0) return launch_on_stream(long_row_kernel<X, R, QUANT>, unsigned(a.N), LONG_THREADS, 0, 1, stream, a);
   const dim3 block(r.threads, r.rows_per_block);
   const unsigned grid = unsigned(((long long)a.N + r.rows_per_block - 1) / r.rows_per_block);

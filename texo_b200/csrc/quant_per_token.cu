@@ -196,17 +196,20 @@ static bool launch(const Args& a, cudaStream_t stream) {
   if (!aligned_rows) {
     const int bytes = a.C <= 32768 ? a.C * int(sizeof(X)) * (FORM == SWIGLU_INTERLEAVED ? 2 : 1) : 0;
     const int room = row::staged_bytes(bytes) * (FORM == SWIGLU_HALVES ? 2 : 1);
-    // (4000 x 11007 BF16: 85 / 51 us for two / four groups per thread)
-    const row::RowPlan r = row::plan_row(a.C, a.N < 512 && a.C <= 8192 ? 1 : 4, block_limit(row::STAGED, 4), 1, false);
+    // (4000 x 11007 BF16: 85 / 48 us for two / four groups per thread; pairs of 128 x 8191, 300 x 8191: 4.1,
+    // 11 us for one, 7.2, 8 for four)
+    row::RowPlan r = row::plan_row(a.C, 1, block_limit(row::STAGED, 1), 1, false);
+    if (!row::at_once(r, a.N, 1536)) r = row::plan_row(a.C, 4, block_limit(row::STAGED, 4), 1, false);
     if (r.units == 0 || room > row::SMEM_LIMIT) return launch_long();
     auto rows = [&](auto* kernel) { return row::launch_staged(kernel, unsigned(a.N), dim3(r.threads), room, stream, a, 1); };
     return r.units == 1 ? rows(row_kernel<X, FORM, row::STAGED, 1>) : rows(row_kernel<X, FORM, row::STAGED, 4>);
   }
-  // One group per thread while rows do not fill the GPU.  Once they do, four: a thread's fixed
-  // work (its place, the reduction, the scale) is spread over more values (8192 x 8192 BF16: 60 /
-  // 41 / 35 us for one / two / four; 4096 x 28672 interleaved pairs: 145 / 120 us for two / four).
-  const row::RowPlan r = a.N < 512 ? row::plan_row(a.C, 1, block_limit(row::ALIGNED, 1), row::MAX_CLUSTER, true)
-                                   : row::plan_row(a.C, 4, block_limit(row::ALIGNED, 4), row::MAX_CLUSTER, true);
+  // 8192 x 8192 BF16: 60 / 41 / 35 us for one / two / four groups per thread; 4096 x 28672
+  // interleaved pairs: 145 / 120 us for two / four; 450 x 4096, 300 x 14336: 4.2, 13.2 us for one,
+  // 4.9, 6.6 for four.  (Clusters hold an SM's second block up.)
+  row::RowPlan r = row::plan_row(a.C, 1, block_limit(row::ALIGNED, 1), row::MAX_CLUSTER, true);
+  if (!row::at_once(r, a.N, r.cluster > 1 ? 1024 : 2048))
+    r = row::plan_row(a.C, 4, block_limit(row::ALIGNED, 4), row::MAX_CLUSTER, true);
   if (r.units == 0 || a.N > 0x7fffffff / r.cluster) return launch_long();
   const dim3 block(r.threads, r.rows_per_block);
   const unsigned grid = unsigned((a.N + r.rows_per_block - 1) / r.rows_per_block) * r.cluster;

@@ -382,6 +382,12 @@ inline RowPlan plan_row(int C, int units, int most_threads, int most_blocks, boo
   p.rows_per_block = p.threads == 32 && p.cluster == 1 && aligned_rows ? 4 : 1;
   return p;
 }
+// Whether all rows are in work at once, on 148 SMs that hold `threads_per_sm` threads each.  Until
+// then the shortest way through a row wins, one group of eight per thread; after that more groups
+// per thread do, which spread a thread's fixed work over more values.
+inline bool at_once(const RowPlan& p, long long N, int threads_per_sm) {
+  return p.units > 0 && N * p.cluster <= 148LL * (threads_per_sm / p.threads);
+}
 constexpr int SMEM_LIMIT = 232448 - 2048;  // (the kernels' own few words are static)
 // Launches a kernel on staged rows; the attribute is set before every launch that needs it, which
 // costs less than keeping track of devices and kernels.
