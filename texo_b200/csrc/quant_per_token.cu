@@ -106,8 +106,11 @@ __device__ __forceinline__ void read_y(uint32_t first, unsigned offset, uint32_t
 }
 
 // Threads of a block at most, and such blocks that an SM has to hold for their latencies to overlap.
-__host__ __device__ constexpr int block_limit(row::Layout layout, int units) {
-  return layout == row::STAGED || units < 4 ? 1024 : 512;
+// Two blocks of 576 leave 56 registers instead of 64, hence three blocks of 352 instead of two: rows
+// of 11008 30.6 -> 24.7 us, as halves 48.5 -> 41.9.  Interleaved pairs want the 64 (4096 x 28672: 120
+// us against 142).
+__host__ __device__ constexpr int block_limit(int form, row::Layout layout, int units) {
+  return layout == row::STAGED || units < 4 ? 1024 : form == SWIGLU_INTERLEAVED ? 512 : 576;
 }
 __host__ __device__ constexpr int blocks_per_sm(row::Layout layout, int units) {
   return layout == row::STAGED || units == 1 ? 1 : 2;
@@ -115,7 +118,7 @@ __host__ __device__ constexpr int blocks_per_sm(row::Layout layout, int units) {
 
 // A block, a warp or (blocks > 1) a cluster per row.  blockDim = (threads, rows of the block).
 template <typename X, int FORM, row::Layout L, int UNITS>
-__global__ void __launch_bounds__(block_limit(L, UNITS), blocks_per_sm(L, UNITS)) row_kernel(const Args a, int blocks) {
+__global__ void __launch_bounds__(block_limit(FORM, L, UNITS), blocks_per_sm(L, UNITS)) row_kernel(const Args a, int blocks) {
   __shared__ unsigned scratch[row::MAX_WARPS], maxima[row::MAX_CLUSTER];
   grid_dependency_trigger();
   row::cluster_started(blocks);
@@ -198,8 +201,8 @@ static bool launch(const Args& a, cudaStream_t stream) {
     const int room = row::staged_bytes(bytes) * (FORM == SWIGLU_HALVES ? 2 : 1);
     // (4000 x 11007 BF16: 85 / 48 us for two / four groups per thread; pairs of 128 x 8191, 300 x 8191: 4.1,
     // 11 us for one, 7.2, 8 for four)
-    row::RowPlan r = row::plan_row(a.C, 1, block_limit(row::STAGED, 1), 1, false);
-    if (!row::at_once(r, a.N, 1536)) r = row::plan_row(a.C, 4, block_limit(row::STAGED, 4), 1, false);
+    row::RowPlan r = row::plan_row(a.C, 1, block_limit(FORM, row::STAGED, 1), 1, false);
+    if (!row::at_once(r, a.N, 1536)) r = row::plan_row(a.C, 4, block_limit(FORM, row::STAGED, 4), 1, false);
     if (r.units == 0 || room > row::SMEM_LIMIT) return launch_long();
     auto rows = [&](auto* kernel) { return row::launch_staged(kernel, unsigned(a.N), dim3(r.threads), room, stream, a, 1); };
     return r.units == 1 ? rows(row_kernel<X, FORM, row::STAGED, 1>) : rows(row_kernel<X, FORM, row::STAGED, 4>);
@@ -207,9 +210,9 @@ static bool launch(const Args& a, cudaStream_t stream) {
   // 8192 x 8192 BF16: 60 / 41 / 35 us for one / two / four groups per thread; 4096 x 28672
   // interleaved pairs: 145 / 120 us for two / four; 450 x 4096, 300 x 14336: 4.2, 13.2 us for one,
   // 4.9, 6.6 for four.  (Clusters hold an SM's second block up.)
-  row::RowPlan r = row::plan_row(a.C, 1, block_limit(row::ALIGNED, 1), row::MAX_CLUSTER, true);
+  row::RowPlan r = row::plan_row(a.C, 1, block_limit(FORM, row::ALIGNED, 1), row::MAX_CLUSTER, true);
   if (!row::at_once(r, a.N, r.cluster > 1 ? 1024 : 2048))
-    r = row::plan_row(a.C, 4, block_limit(row::ALIGNED, 4), row::MAX_CLUSTER, true);
+    r = row::plan_row(a.C, 4, block_limit(FORM, row::ALIGNED, 4), row::MAX_CLUSTER, true);
   if (r.units == 0 || a.N > 0x7fffffff / r.cluster) return launch_long();
   const dim3 block(r.threads, r.rows_per_block);
   const unsigned grid = unsigned((a.N + r.rows_per_block - 1) / r.rows_per_block) * r.cluster;
