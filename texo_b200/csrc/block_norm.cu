@@ -124,9 +124,13 @@ struct Scratch {
   unsigned max[row::MAX_WARPS];
 };
 
-// A block (or a warp) per row.  blockDim = (threads of a row, rows of the block).
-template <typename X, typename R, bool QUANT, row::Layout L, int UNITS>
-__global__ void __launch_bounds__(1024) row_kernel(const Args a) {
+// A block (or a warp) per row.  blockDim = (threads of a row, rows of the block), LIMIT threads at most.
+// Two blocks of 576 leave 56 registers instead of 64, hence three blocks of 384 on an SM instead of
+// two (4096 x 6144 BF16, both norms, gate, quantised: 52.5 -> 42.4 us; 5999: 88.5 -> 73.2); where that
+// spills (wider residual, y not quantised: 4096 x 8192 67.6 -> 70.4 us) it is not done.
+constexpr int SHORT = 576;
+template <typename X, typename R, bool QUANT, row::Layout L, int UNITS, int LIMIT>
+__global__ void __launch_bounds__(LIMIT, LIMIT == SHORT ? 2 : 1) row_kernel(const Args a) {
   __shared__ Scratch scratch;
   grid_dependency_trigger();
   const long long row_number = (long long)blockIdx.x * blockDim.y + threadIdx.y;
@@ -262,13 +266,20 @@ static bool launch(const Args& a, cudaStream_t stream) {
   if (r.units == 0) return launch_on_stream(long_row_kernel<X, R, QUANT>, unsigned(a.N), LONG_THREADS, 0, 1, stream, a);
   const dim3 block(r.threads, r.rows_per_block);
   const unsigned grid = unsigned(((long long)a.N + r.rows_per_block - 1) / r.rows_per_block);
-  if (aligned_rows)
-    return r.units == 1
-               ? launch_on_stream(row_kernel<X, R, QUANT, row::ALIGNED, 1>, grid, block, 0, 1, stream, a)
-               : launch_on_stream(row_kernel<X, R, QUANT, row::ALIGNED, 2>, grid, block, 0, 1, stream, a);
+  constexpr bool HAS_SHORT = QUANT || sizeof(R) == sizeof(X);
+  if (aligned_rows) {
+    auto rows = [&](auto* kernel) { return launch_on_stream(kernel, grid, block, 0, 1, stream, a); };
+    if (r.units == 1) return rows(row_kernel<X, R, QUANT, row::ALIGNED, 1, 1024>);
+    if constexpr (HAS_SHORT)
+      if (r.threads <= SHORT) return rows(row_kernel<X, R, QUANT, row::ALIGNED, 2, SHORT>);
+    return rows(row_kernel<X, R, QUANT, row::ALIGNED, 2, 1024>);
+  }
   const int room = row::staged_bytes((long long)a.C * sizeof(X)) + row::staged_bytes((long long)a.C * sizeof(R));
-  return r.units == 1 ? row::launch_staged(row_kernel<X, R, QUANT, row::STAGED, 1>, grid, block, room, stream, a)
-                      : row::launch_staged(row_kernel<X, R, QUANT, row::STAGED, 2>, grid, block, room, stream, a);
+  auto rows = [&](auto* kernel) { return row::launch_staged(kernel, grid, block, room, stream, a); };
+  if (r.units == 1) return rows(row_kernel<X, R, QUANT, row::STAGED, 1, 1024>);
+  if constexpr (HAS_SHORT)
+    if (r.threads <= SHORT) return rows(row_kernel<X, R, QUANT, row::STAGED, 2, SHORT>);
+  return rows(row_kernel<X, R, QUANT, row::STAGED, 2, 1024>);
 }
 
 template <bool QUANT>

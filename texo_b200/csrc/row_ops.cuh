@@ -220,7 +220,7 @@ struct Spread {
 // Rows that start anywhere: the bytes move in aligned 16-byte granules between global and shared
 // memory, and are shifted by the row's offset (the same for the whole row) between shared memory
 // and registers.  Loads and stores of single values took twice as long (quant_per_token on 4000 x
-// 11007 BF16: 106 us against 51).
+// 11007 BF16: 106 us against 49).
 
 // A staged input's room: its granules, and one more that the last shift reads.
 __host__ __device__ constexpr int staged_bytes(long long bytes) { return int((bytes + 15) / 16 * 16 + 48); }
