@@ -429,8 +429,8 @@ def test_swiglu_quant_matches_64_bits(ops, shape, x_type, interleaved):
     gate, up = (gu[:, 0::2], gu[:, 1::2]) if interleaved else (gu[:, :F], gu[:, F:])
     gate, up = gate.double(), up.double()
     y = gate * torch.sigmoid(gate) * up
-    # __expf is off by 2 + 1.16 |gate| ulps (2 U each), which the quotient sees at most whole;
-    # the sum 1, the quotient 2 ulps, the product 1
+    # (in U) e^-gate = 2^(-gate log2 e): the exponent's rounding and its constant's 1.23 |gate|, the power
+    # two ulps = 4; the sum 1, the reciprocal one ulp = 2, the products 1 each
     dy = y.abs() * (2 * (2 + 1.16 * gate.abs()) + 1 + 4 + 1) * U + 2.0 ** -126
     q, s = ops.swiglu_quant_per_token(gu, interleaved=interleaved)
     check_quantised(q, s, y, dy)

@@ -75,10 +75,13 @@ struct TokenScale {
   float scale;
   float hi, lo;  // 1 / scale in two terms; hi = 0: q is zero whatever y is
 };
-// Quotients by multiplication: scale with a reciprocal and corrections by exact residuals, y / scale
-// (below) with a reciprocal of 48 bits, which rounds like the quotient but for one in 2^23.  A
-// few instructions that every thread can afford, where IEEE divisions take an eighth of a short
-// row's time.
+// Quotients by multiplication (Newton-Raphson on 1/b and on a/b with residuals that a fused
+// multiply-add gives exactly; Markstein, "Computation of elementary functions on the IBM RISC System/6000
+// processor", 1990).  scale: q0 = a * RN(1/127) is within two ulps of a/127; q1 = q0 + (a - 127 q0) *
+// RN(1/127) within one; the same step from there rounds correctly.  y / scale: one Newton step takes
+// the approximate reciprocal r to hi = r + (1 - scale r) r, within half an ulp and a little; lo = (1 - scale hi)
+// hi is the rest, and hi + lo is within 2^-47 of 1/scale.  A few instructions that every thread can
+// afford, where divisions take an eighth of a short row's time.
 __device__ __forceinline__ TokenScale token_scale(float amax) {
   TokenScale s;
   if (__float_as_uint(amax) >= 0x7f800000u) {
