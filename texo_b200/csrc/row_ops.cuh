@@ -225,8 +225,10 @@ struct Spread {
 // and registers.  Loads and stores of single values took twice as long (quant_per_token on 4000 x
 // 11007 BF16: 106 us against 49).
 
-// A staged input's room: its granules, and one more that the last shift reads.
-__host__ __device__ constexpr int staged_bytes(long long bytes) { return int((bytes + 15) / 16 * 16 + 48); }
+// A staged input's room: its granules and four more.  The last group's shift reads farthest past the row's
+// end, of interleaved FP32 pairs (C = 8 k + 1: the group's second eight values start 24 bytes behind the
+// row's end and come in three granules, 72 bytes in all; 44 in the 16-bit types).
+__host__ __device__ constexpr int staged_bytes(long long bytes) { return int((bytes + 15) / 16 * 16 + 64); }
 
 // Starts copying the granules that hold [src, src + bytes) to shared memory.  Bytes of granules that reach
 // outside [begin, end) are loaded singly.
