@@ -1,0 +1,63 @@
+"""GPU tests of the dynamic-quantisation operators at the ends of their ranges: values, sizes,
+errors of other calls, and the paths of the product that only large problems take.  Helpers and the
+counting of roundings are those of test_per_token_gpu.py."""
+import pytest
+
+from tests.test_per_token_gpu import (BF16, F16, F32, U, check_quantised, dtype, generator, mm_expected, mm_inputs,
+                                      assert_within, ops)  # noqa: F401  (ops is a fixture)
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+# ------------------------------------------------------------------ SwiGLU far from zero
+def far_rows(F, x_type, seed):
+    """gate, up [8, F]: rows whose outputs are finite although exp(-gate), or gate * up, is not."""
+    g = generator(seed)
+
+    def between(lo, hi):
+        return (torch.rand(F, generator=g, device="cuda") * (hi - lo) + lo).to(dtype(x_type))
+
+    big = 6e4 if x_type == F16 else 1e38  # (2^126.2; an f16 gate of -87 and this make 5e-33)
+    gates = [between(-104, -86), between(-170, -100), between(-20, -1), between(-90, -84), between(-300, -87),
+             between(-8, 8), between(-90, 8), between(-88.8, -86.4)]
+    ups = [between(0.5 * big, big), between(0.9 * big, big), between(0.5 * big, big), between(-2, 2), between(-2, 2),
+           between(-2, 2), between(-1, 1) * min(big, 1e6), between(-big, big)]
+    return torch.stack(gates), torch.stack(ups)
+
+
+@pytest.mark.parametrize("F", [1, 2, 9, 64, 65, 1024, 1025, 8192, 8191, 20001, 28672, 40001])
+@pytest.mark.parametrize("x_type", [F16, BF16, F32])
+@pytest.mark.parametrize("interleaved", [True, False])
+def test_swiglu_where_the_exponential_overflows(ops, F, x_type, interleaved):
+    """In U, relative to y: 1.23 |gate| + 9 as the kernel counts them; gates below -80: the exponent
+    of e^(gate / 2) is exact, the function two ulps (4), two of it, three products: 11.  The absolute
+    2^-114 stands for gates below -174, where e^(gate / 2) is subnormal."""
+    gate, up = far_rows(F, x_type, F)
+    x = torch.stack([gate, up], dim=2).reshape(8, 2 * F) if interleaved else torch.cat([gate, up], dim=1)
+    g64, u64 = gate.double(), up.double()
+    y = g64 / (1 + torch.exp(-g64)) * u64
+    assert bool((y.abs().amax(dim=1) < 3e38).all())
+    dy = y.abs() * (1.24 * g64.abs().clamp_max(90) + 12) * U + 2.0 ** -114
+    q, s = ops.swiglu_quant_per_token(x.contiguous(), interleaved=interleaved)
+    check_quantised(q, s, y, dy)
+    if x_type != F16:
+        assert bool((q[:3].abs().amax(dim=1) == 127).all())  # rows of far gates have values
+    part = x[5:6].contiguous()
+    q1, s1 = ops.swiglu_quant_per_token(part, interleaved=interleaved)
+    assert torch.equal(q1[0], q[5]) and torch.equal(s1[0], s[5])
+
+
+@pytest.mark.parametrize("F", [64, 65, 8192, 40001])
+@pytest.mark.parametrize("x_type", [F16, BF16, F32])
+def test_swiglu_of_values_that_are_not_finite(ops, F, x_type):
+    inf, nan = float("inf"), float("nan")
+    rows = [(1.0, 1.0), (nan, 1.0), (1.0, nan), (inf, 1.0), (-inf, 1.0), (1.0, inf), (-100.0, inf), (-inf, 0.0), (2.0, -3.0)]
+    gate = torch.full((len(rows), F), 0.5, dtype=dtype(x_type), device="cuda")
+    up = torch.full_like(gate, 0.25)
+    for r, (a, b) in enumerate(rows):
+        gate[r, F - 1], up[r, F - 1] = a, b
+    x = torch.cat([gate, up], dim=1)
+    q, s = ops.swiglu_quant_per_token(x, interleaved=False)
+    assert s.isnan().tolist() == [False] + [True] * 7 + [False]
+    assert not bool(q[1:8].any()) and bool((q[0] != 0).all())

@@ -9,6 +9,7 @@
 // One scale per row needs the row's maximum before its first output, so the row stays in
 // registers between the two: bound by HBM bandwidth, each byte crosses once (row_ops.cuh).
 // Long rows are shared by a cluster of blocks that exchange their maxima.
+#include <cmath>
 #include <cstdint>
 #include <cuda_runtime.h>
 
@@ -30,52 +31,68 @@ struct Args {
   long long stride;  // elements between rows of x
 };
 
-// gate and up are never multiplied first: their product can overflow where the result does not.
-// e^-gate is 2^(-gate log2 e).  In multiples of U = 2^-24, relative to the value: rounding log2 e and
-// the product moves the exponent by 1.23 parts of itself, hence the power by 1.23 |gate|; PTX allows
-// ex2.approx 4 (two ulps) and rcp.approx 2; the sum and the two products take 1 each.  Together
-// 9 + 1.23 |gate|, a thousandth of the quantiser's half step for gates of a hundred.  (The correctly
-// rounded functions: 181 us where this form takes 120, 4096 x 28672 BF16 pairs, and 20 of its
-// 117,440,512 outputs the other way from a tie.)  Both instructions flush subnormals, which saves
-// the scaling around them: a denominator beyond 2^126 (gate < -87) makes silu(gate) 0, less than
-// 2^-118 away from what it is.
+// y = gate up / (1 + e^-gate), and e^-gate = 2^(-gate log2 e).  Errors in multiples of U = 2^-24,
+// relative to the value: rounding log2 e and its product moves the exponent by 1.23 parts of itself, hence the
+// power by 1.23 |gate|; PTX allows ex2.approx 4 (two ulps) and rcp.approx 2; the sum takes 1, the
+// products 1 each, the first one none where the inputs have 16 bits.  Together 9 + 1.23 |gate|, far
+// below the quantiser's half step: 20 of 117,440,512 outputs fall on the other side of a tie than with
+// expf and an IEEE division, which take 181 us instead of 120 (4096 x 28672 BF16 pairs).
+// Both instructions flush subnormals, which saves the scaling around them: a denominator beyond 2^126
+// (gate < -87.3) would make y zero, where a large `up` may make it any value.  And gate * up can
+// overflow where y does not.  Rows with either are done again (careful_row below).
 constexpr float LOG2_E = 1.44269504f;
+constexpr float LOWEST_GATE = -87.f;
 __device__ __forceinline__ float swiglu(float gate, float up) {
   float e, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmul_rn(gate, -LOG2_E)));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__fadd_rn(1.f, e)));
-  return gate * r * up;
+  return __fmul_rn(r, __fmul_rn(gate, up));
 }
-
-// The same of eight, in packed arithmetic (and the same bits).
-__device__ __forceinline__ void swiglu8(const float (&gate)[8], const float (&up)[8], float (&y)[8]) {
-  float t[8];
+// The same of eight, in packed arithmetic (and the same bits), and the lowest gate.
+__device__ __forceinline__ void swiglu8(const float (&gate)[8], const float (&up)[8], float (&y)[8], float& lowest) {
+  float t[8], product[8];
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) asm("min.f32 %0, %0, %1, %2;" : "+f"(lowest) : "f"(gate[j]), "f"(gate[j + 1]));
   row::mul8(t, gate, -LOG2_E);
 #pragma unroll
   for (int j = 0; j < 8; ++j) asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(t[j]));
   row::fma8(t, t, 1.f, 1.f);
 #pragma unroll
   for (int j = 0; j < 8; ++j) asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(t[j]));
-  row::mul8(t, gate, t);
-  row::mul8(y, t, up);
+  row::mul8(product, gate, up);
+  row::mul8(y, t, product);
 }
-// Eight outputs from sixteen interleaved inputs.
-__device__ __forceinline__ void swiglu_pairs(const float (&lo)[8], const float (&hi)[8], float (&y)[8]) {
-  const float gate[8] = {lo[0], lo[2], lo[4], lo[6], hi[0], hi[2], hi[4], hi[6]};
-  const float up[8] = {lo[1], lo[3], lo[5], lo[7], hi[1], hi[3], hi[5], hi[7]};
-  swiglu8(gate, up, y);
+// For any finite gate and up.  Below -80, 1 + e^-gate is e^-gate, and y = (gate h) (h up) with h =
+// e^(gate / 2): no factor leaves the range unless y does (h is subnormal below -174, where |y| < 2^-115
+// whatever up is, a hundredth of the smallest scale).  Where the product overflows the quotient comes first.
+__device__ __forceinline__ float careful_swiglu(float gate, float up) {
+  if (gate < -80.f) {
+    const float h = expf(0.5f * gate);
+    return (gate * h) * (h * up);
+  }
+  const float y = swiglu(gate, up);
+  return fabsf(y) < INFINITY ? y : gate / (1.f + expf(-gate)) * up;
 }
 
-// Group i of an aligned row in global memory, as y; values past the end are zero.
+// Eight outputs from sixteen interleaved inputs.
+__device__ __forceinline__ void swiglu_pairs(const float (&lo)[8], const float (&hi)[8], float (&y)[8], float& lowest) {
+  const float gate[8] = {lo[0], lo[2], lo[4], lo[6], hi[0], hi[2], hi[4], hi[6]};
+  const float up[8] = {lo[1], lo[3], lo[5], lo[7], hi[1], hi[3], hi[5], hi[7]};
+  swiglu8(gate, up, y, lowest);
+}
+
+// Group i of an aligned row in global memory, as y; values past the end are zero.  `lowest` goes down to its
+// lowest gate.
 template <typename X, int FORM>
-__device__ __forceinline__ void load_y(const X* x, const row::Spread<row::ALIGNED>& s, int i, float (&y)[8]) {
+__device__ __forceinline__ void load_y(const X* x, const row::Spread<row::ALIGNED>& s, int i, float (&y)[8],
+                                       float& lowest) {
   if (FORM == PLAIN) {
     s.template load<true>(x, i, y);
   } else if (FORM == SWIGLU_HALVES) {
     float g[8], u[8];
     s.template load<true>(x, i, g);
     s.template load<true>(x + s.C, i, u);
-    swiglu8(g, u, y);
+    swiglu8(g, u, y, lowest);
   } else {
     // the sixteen inputs of eight outputs: two groups of a row of 2 C values
     const row::Spread<row::ALIGNED> wide = {0, 1, 2 * s.C};
@@ -83,13 +100,13 @@ __device__ __forceinline__ void load_y(const X* x, const row::Spread<row::ALIGNE
     const int c = s.at(i, 0);
     wide.template load<true>(x, c / 4, lo);
     wide.template load<true>(x, c / 4 + 1, hi);
-    swiglu_pairs(lo, hi, y);
+    swiglu_pairs(lo, hi, y, lowest);
   }
 }
 // The same of a staged row: `first` holds x (or the gates, `second` the ups).
 template <typename X, int FORM>
 __device__ __forceinline__ void read_y(uint32_t first, unsigned offset, uint32_t second, unsigned second_offset,
-                                       const row::Spread<row::STAGED>& s, int i, float (&y)[8]) {
+                                       const row::Spread<row::STAGED>& s, int i, float (&y)[8], float& lowest) {
   if (s.at(i, 0) >= s.C) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) y[j] = 0.f;
@@ -99,13 +116,13 @@ __device__ __forceinline__ void read_y(uint32_t first, unsigned offset, uint32_t
     float lo[8], hi[8];
     row::read_staged<X>(first, offset, 2 * s.at(i, 0), lo);
     row::read_staged<X>(first, offset, 2 * s.at(i, 0) + 8, hi);
-    swiglu_pairs(lo, hi, y);
+    swiglu_pairs(lo, hi, y, lowest);
   } else {
     row::read_staged<X>(first, offset, s.at(i, 0), y);
     if (FORM == SWIGLU_HALVES) {
       float u[8];
       row::read_staged<X>(second, second_offset, s.at(i, 0), u);
-      swiglu8(y, u, y);
+      swiglu8(y, u, y, lowest);
     }
   }
   s.mask(i, y);  // (what lies past the row's end is arbitrary)
@@ -122,10 +139,39 @@ __host__ __device__ constexpr int blocks_per_sm(row::Layout layout, int units) {
   return layout == row::STAGED || units == 1 ? 1 : 2;
 }
 
+// A row whose y is computed twice, value by value, by `threads` threads in `blocks` blocks.
+template <typename X, int FORM>
+__device__ __forceinline__ void row_in_passes(const Args& a, long long n, int t, int threads, int blocks, unsigned* scratch,
+                                              unsigned* maxima) {
+  const X* x = static_cast<const X*>(a.x) + n * a.stride;
+  auto y_at = [&](int c) {
+    if (FORM == PLAIN) return row::to_float(x[c]);
+    const size_t g = FORM == SWIGLU_INTERLEAVED ? 2 * size_t(c) : c;
+    const size_t u = FORM == SWIGLU_INTERLEAVED ? 2 * size_t(c) + 1 : size_t(a.C) + c;
+    return careful_swiglu(row::to_float(x[g]), row::to_float(x[u]));
+  };
+  float amax = 0.f;
+  for (int c = t; c < a.C; c += threads) amax = row::max_abs(amax, y_at(c));
+  amax = row::cluster_max(amax, scratch, threadIdx.x, blockDim.x / 32, maxima, blocks);
+  const row::TokenScale scale = row::token_scale(amax);
+  if (t == 0) a.scale[n] = scale.scale;
+  int8_t* q = a.q + size_t(n) * a.C;
+  for (int c = t; c < a.C; c += threads) q[c] = row::quantise(y_at(c), scale);
+}
+// Once more, for a row of SwiGLU products with a far gate or one that is not finite.  The row's number
+// comes from the special registers again, which keeps it and the row's addresses out of the registers
+// until here (4096 x 28672 BF16 pairs 119.7 us, handed over 126.6).
+template <typename X, int FORM>
+__device__ __forceinline__ void careful_row(const Args& a, int blocks, unsigned* scratch, unsigned* maxima) {
+  row::cluster_started(blocks);
+  const long long n = (long long)cluster_id() * blockDim.y + threadIdx.y;
+  row_in_passes<X, FORM>(a, n, int(cluster_ctarank() * blockDim.x + threadIdx.x), blocks * blockDim.x, blocks, scratch, maxima);
+}
+
 // A block, a warp or (blocks > 1) a cluster per row.  blockDim = (threads, rows of the block).
 template <typename X, int FORM, row::Layout L, int UNITS>
 __global__ void __launch_bounds__(block_limit(FORM, L, UNITS), blocks_per_sm(L, UNITS)) row_kernel(const Args a, int blocks) {
-  __shared__ unsigned scratch[row::MAX_WARPS], maxima[row::MAX_CLUSTER];
+  __shared__ unsigned scratch[2][row::MAX_WARPS], maxima[2][row::MAX_CLUSTER];
   grid_dependency_trigger();
   row::cluster_started(blocks);
   const int part = int(cluster_ctarank());  // of the row
@@ -136,10 +182,10 @@ __global__ void __launch_bounds__(block_limit(FORM, L, UNITS), blocks_per_sm(L, 
   const X* x = static_cast<const X*>(a.x) + n * a.stride;
   int8_t* q = a.q + size_t(n) * a.C;
   grid_dependency_wait();
-  float y[UNITS][8];
+  float y[UNITS][8], lowest = 0.f;
   if constexpr (L == row::ALIGNED) {
 #pragma unroll
-    for (int i = 0; i < UNITS; ++i) load_y<X, FORM>(x, s, i, y[i]);
+    for (int i = 0; i < UNITS; ++i) load_y<X, FORM>(x, s, i, y[i], lowest);
   } else {  // a block per row; x's room takes q afterwards
     extern __shared__ __align__(16) uint8_t staging[];
     const uintptr_t begin = reinterpret_cast<uintptr_t>(a.x);
@@ -152,17 +198,21 @@ __global__ void __launch_bounds__(block_limit(FORM, L, UNITS), blocks_per_sm(L, 
     row::fetched();
 #pragma unroll
     for (int i = 0; i < UNITS; ++i)
-      read_y<X, FORM>(to, unsigned(first & 15), to_second, unsigned(second & 15), s, i, y[i]);
+      read_y<X, FORM>(to, unsigned(first & 15), to_second, unsigned(second & 15), s, i, y[i], lowest);
     __syncthreads();
     q = reinterpret_cast<int8_t*>(staging);
   }
-  float amax = 0.f;
+  float amax = lowest < LOWEST_GATE ? INFINITY : 0.f;
 #pragma unroll
   for (int i = 0; i < UNITS; ++i) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) amax = row::max_abs(amax, y[i][j]);
   }
-  amax = row::cluster_max(amax, scratch, t, threads / 32, maxima, blocks);
+  amax = row::cluster_max(amax, scratch[0], t, threads / 32, maxima[0], blocks);
+  if (FORM != PLAIN && !(amax < INFINITY)) {  // the same for all threads of the row
+    careful_row<X, FORM>(a, blocks, scratch[1], maxima[1]);
+    return;
+  }
   const row::TokenScale scale = row::token_scale(amax);
   if (s.t == 0) a.scale[n] = scale.scale;
 #pragma unroll
@@ -173,28 +223,14 @@ __global__ void __launch_bounds__(block_limit(FORM, L, UNITS), blocks_per_sm(L, 
   }
 }
 
-// Rows that the registers do not hold: y is computed twice.
+// Rows that the registers do not hold.
 constexpr int LONG_THREADS = 1024;
 template <typename X, int FORM>
 __global__ void __launch_bounds__(LONG_THREADS) long_row_kernel(const Args a) {
   __shared__ unsigned scratch[row::MAX_WARPS];
   grid_dependency_trigger();
   grid_dependency_wait();
-  const long long n = blockIdx.x;
-  const X* x = static_cast<const X*>(a.x) + n * a.stride;
-  auto y_at = [&](int c) {
-    if (FORM == PLAIN) return row::to_float(x[c]);
-    const size_t g = FORM == SWIGLU_INTERLEAVED ? 2 * size_t(c) : c;
-    const size_t u = FORM == SWIGLU_INTERLEAVED ? 2 * size_t(c) + 1 : size_t(a.C) + c;
-    return swiglu(row::to_float(x[g]), row::to_float(x[u]));
-  };
-  float amax = 0.f;
-  for (int c = threadIdx.x; c < a.C; c += LONG_THREADS) amax = row::max_abs(amax, y_at(c));
-  amax = row::row_max(amax, scratch, threadIdx.x, LONG_THREADS / 32);
-  const row::TokenScale scale = row::token_scale(amax);
-  if (threadIdx.x == 0) a.scale[n] = scale.scale;
-  int8_t* q = a.q + size_t(n) * a.C;
-  for (int c = threadIdx.x; c < a.C; c += LONG_THREADS) q[c] = row::quantise(y_at(c), scale);
+  row_in_passes<X, FORM>(a, blockIdx.x, threadIdx.x, LONG_THREADS, 1, scratch, nullptr);
 }
 
 template <typename X, int FORM>
