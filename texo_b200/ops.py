@@ -27,6 +27,12 @@ def _check_cuda(name: str, t: torch.Tensor, dtype: torch.dtype) -> None:
         raise ValueError(f"{name} must be contiguous and row-major")
 
 
+def _check_sizes(*sizes: int) -> None:
+    """The library takes sizes as C ints, of which ctypes would pass the low 32 bits."""
+    if max(sizes) > 0x7fffffff:
+        raise ValueError("sizes must be below 2^31")
+
+
 class _DefaultStreamOrder:
     """The library issues work on the legacy default stream (reference contract).  When the
     caller's current torch stream is another one, order the two around the call."""
@@ -58,6 +64,7 @@ def mm_int8(A: torch.Tensor, B: torch.Tensor, scale_A: float, scale_B: float, sc
         raise ValueError(f"shape mismatch: A {tuple(A.shape)} B {tuple(B.shape)}")
     M, K = A.shape
     N = B.shape[1]
+    _check_sizes(M, N, K)
     if M <= 0 or N <= 0:
         raise ValueError("M and N must be positive")
     if out is None:
@@ -86,6 +93,7 @@ def mm_int8_per_channel(A: torch.Tensor, B: torch.Tensor, scale_A: float, scale_
         raise ValueError(f"shape mismatch: A {tuple(A.shape)} B {tuple(B.shape)}")
     M, K = A.shape
     N = B.shape[1]
+    _check_sizes(M, N, K)
     if M <= 0 or N <= 0 or tuple(scale_B.shape) != (N,):
         raise ValueError("M, N must be positive and scale_B must be [N]")
     if zero_point_B is not None:
@@ -119,6 +127,7 @@ def mm_int8_swiglu(A: torch.Tensor, B_gu: torch.Tensor, scale_A: float, scale_ga
         raise ValueError(f"shape mismatch: A {tuple(A.shape)} B_gu {tuple(B_gu.shape)}")
     M, K = A.shape
     F = B_gu.shape[1] // 2
+    _check_sizes(M, F, K)
     if M <= 0 or F <= 0:
         raise ValueError("M and F must be positive")
     if out is None:
@@ -145,6 +154,7 @@ def mm_int8_dequant(A: torch.Tensor, B: torch.Tensor, scale_A: float, scale_B: f
         raise ValueError(f"shape mismatch: A {tuple(A.shape)} B {tuple(B.shape)}")
     M, K = A.shape
     N = B.shape[1]
+    _check_sizes(M, N, K)
     if M <= 0 or N <= 0:
         raise ValueError("M and N must be positive")
     if out is None:
@@ -168,6 +178,7 @@ def mm_int4(x: torch.Tensor, w_q: torch.Tensor, scales: torch.Tensor, group_size
     _check_cuda("scales", scales, torch.float16)
     M, K = x.shape
     N = w_q.shape[0]
+    _check_sizes(M, N, K)
     if K % 2 or w_q.shape[1] != K // 2:
         raise ValueError("w_q must be [N, K/2] with even K")
     if group_size <= 0 or K % group_size or tuple(scales.shape) != (N, K // group_size):
@@ -194,6 +205,7 @@ def mm_int4a8(A: torch.Tensor, w_q: torch.Tensor, scale_A: float, scale_B: float
         raise ValueError("A and w_q must be matrices")
     M, K = A.shape
     N = w_q.shape[0]
+    _check_sizes(M, N, K)
     if K % 2 or w_q.shape[1] != K // 2:
         raise ValueError("w_q must be [N, K/2] with even K")
     if M <= 0 or N <= 0:
@@ -224,6 +236,7 @@ def mm_int4a8_per_channel(A: torch.Tensor, w_q: torch.Tensor, scale_A: float, sc
         raise ValueError("A and w_q must be matrices")
     M, K = A.shape
     N = w_q.shape[0]
+    _check_sizes(M, N, K)
     if K % 2 or w_q.shape[1] != K // 2:
         raise ValueError("w_q must be [N, K/2] with even K")
     if M <= 0 or N <= 0 or tuple(scale_B.shape) != (N,):
@@ -259,6 +272,7 @@ def mm_int8_per_group(A: torch.Tensor, B: torch.Tensor, group_size: int, scale_A
         raise ValueError("A must be [M, K] and B [K, N]")
     M, K = A.shape
     N = B.shape[1]
+    _check_sizes(M, N, K)
     if M <= 0 or N <= 0 or K <= 0 or group_size <= 0 or K % group_size:
         raise ValueError("M, N, K must be positive and group_size must divide K")
     if tuple(scale_B.shape) != (K // group_size, N):
@@ -284,6 +298,7 @@ def mm_int4a8_per_group(A: torch.Tensor, w_q: torch.Tensor, group_size: int, sca
         raise ValueError("A and w_q must be matrices")
     M, K = A.shape
     N = w_q.shape[0]
+    _check_sizes(M, N, K)
     if K <= 0 or K % 2 or w_q.shape[1] != K // 2:
         raise ValueError("w_q must be [N, K/2] with even K > 0")
     if M <= 0 or N <= 0 or group_size <= 0 or K % group_size:
@@ -305,6 +320,7 @@ def dequantization(X: torch.Tensor, S: torch.Tensor, T: int,
     _check_cuda("X", X, torch.float32)
     _check_cuda("S", S, torch.float32)
     M, N = X.shape
+    _check_sizes(M, N, T)
     if T <= 0 or tuple(S.shape) != ((M + T - 1) // T, (N + T - 1) // T):
         raise ValueError("S must be [ceil(M/T), ceil(N/T)]")
     if out is None:
@@ -323,6 +339,7 @@ def _check_norm_inputs(x, residual, weight):
     _check_cuda("weight", weight, torch.float32)
     if x.dim() != 2 or residual.shape != x.shape or tuple(weight.shape) != (x.shape[1],):
         raise ValueError("x, residual must be [N, C] and weight [C]")
+    _check_sizes(*x.shape)
     if x.shape[0] <= 0 or x.shape[1] <= 0:
         raise ValueError("N and C must be positive")
 
@@ -389,6 +406,7 @@ def mm_int8_host(A_host: torch.Tensor, B_host: torch.Tensor, C_host: torch.Tenso
             raise ValueError(f"{name} must be a contiguous CPU int8 tensor")
     M, K = A_host.shape
     N = B_host.shape[1]
+    _check_sizes(M, N, K)
     if B_host.shape[0] != K or tuple(C_host.shape) != (M, N):
         raise ValueError("shape mismatch")
     rc = _lib.load().texo_mm_int8_solve_host(A_host.data_ptr(), B_host.data_ptr(), C_host.data_ptr(),
@@ -407,6 +425,7 @@ class Int8Weights:
         _check_cuda("B", B, torch.int8)
         if B.dim() != 2 or B.shape[0] <= 0 or B.shape[1] <= 0:
             raise ValueError("B must be a non-empty [K, N] matrix")
+        _check_sizes(*B.shape)
         self.B = B  # keeps the storage alive
         self.K, self.N = B.shape
         self._lib = _lib.load()
@@ -424,6 +443,7 @@ class Int8Weights:
         if A.dim() != 2 or A.shape[1] != self.K:
             raise ValueError(f"A must be [M, {self.K}]")
         M = A.shape[0]
+        _check_sizes(M)
         if out is None:
             out = torch.empty((M, self.N), dtype=torch.int8, device=A.device)
         else:
@@ -526,6 +546,7 @@ def mm_int8_per_token(A: torch.Tensor, B: torch.Tensor, scale_A: torch.Tensor, s
         raise ValueError(f"shape mismatch: A {tuple(A.shape)} B {tuple(B.shape)}")
     M, K = A.shape
     N = B.shape[1]
+    _check_sizes(M, N, K)
     if N <= 0 or scale_A.shape != (M,) or scale_B.shape != (N,):
         raise ValueError("N must be positive, scale_A must be [M] and scale_B [N]")
     if bias is not None:
@@ -557,6 +578,7 @@ def _block_norm(quant, x, residual, weight, eps, post_weight, gate, residual_sca
     if len(shape) != 2 or residual.shape != shape or shape[1] <= 0 or weight.shape != (shape[1],):
         raise ValueError("x, residual must be [N, C] with C > 0 and weight [C]")
     N, C = shape
+    _check_sizes(N, C)
     if residual_code != x_code and residual_code != 2:
         raise ValueError("residual must have x's type or float32")
     if weight_code != x_code and weight_code != 2:
@@ -649,6 +671,7 @@ def quant_per_token(x: torch.Tensor, out: torch.Tensor | None = None,
     that holds a NaN or an infinity gets scale NaN and q = 0."""
     code = _check_rows("x", x)
     N, C = x.shape
+    _check_sizes(N, C)
     q, scale = _quantised(x, N, C, out, scale_out)
     if N > 0:
         _call_on_stream("texo_quant_per_token_solve", x, (q, scale), x.data_ptr(), q.data_ptr(), scale.data_ptr(),
@@ -663,6 +686,7 @@ def swiglu_quant_per_token(gate_up: torch.Tensor, interleaved: bool = True, out:
     int8 [N,F], scale float32 [N])."""
     code = _check_rows("gate_up", gate_up)
     N, width = gate_up.shape
+    _check_sizes(N, width)
     if width % 2:
         raise ValueError("gate_up must have an even number of columns")
     q, scale = _quantised(gate_up, N, width // 2, out, scale_out)
