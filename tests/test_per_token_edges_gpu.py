@@ -61,3 +61,31 @@ def test_swiglu_of_values_that_are_not_finite(ops, F, x_type):
     q, s = ops.swiglu_quant_per_token(x, interleaved=False)
     assert s.isnan().tolist() == [False] + [True] * 7 + [False]
     assert not bool(q[1:8].any()) and bool((q[0] != 0).all())
+
+
+# ------------------------------------------------------------------ errors of other calls
+@pytest.mark.parametrize("K", [0, 40, 131072])
+def test_an_error_of_the_callers_is_left_alone(ops, K):
+    """An error code that an earlier CUDA call of the caller's left behind is neither taken for the
+    product's own nor cleared, whichever kernel runs (K = 0 and K = 2^17: the SIMT one)."""
+    import ctypes
+
+    M, N = 3, 32
+    A, B, sa, sb, bias = mm_inputs(M, N, K, 6) if K else (
+        torch.empty((M, 0), dtype=torch.int8, device="cuda"), torch.empty((0, N), dtype=torch.int8, device="cuda"),
+        torch.ones(M, device="cuda"), torch.ones(N, device="cuda"), torch.ones(N, device="cuda"))
+    want = ops.mm_int8_per_token(A, B, sa, sb, bias, out_dtype=torch.float32)
+    out = torch.full_like(want, 7.0)
+    torch.cuda.synchronize()
+    runtime = ctypes.CDLL("libcudart.so.12")
+    value = ctypes.c_int()
+    invalid_device = 101
+    assert runtime.cudaGetLastError() == 0
+    assert runtime.cudaDeviceGetAttribute(ctypes.byref(value), 1, 4096) == invalid_device  # no such device
+    try:
+        assert runtime.cudaPeekAtLastError() == invalid_device
+        ops.mm_int8_per_token(A, B, sa, sb, bias, out_dtype=torch.float32, out=out)
+        assert runtime.cudaPeekAtLastError() == invalid_device
+    finally:
+        runtime.cudaGetLastError()
+    assert torch.equal(out, want)

@@ -1047,12 +1047,21 @@ static bool launch_generic(const int8_t* A, const int8_t* B, Y* out, int M, int 
     const int rows = std::min(M - m0, ROWS);
     const dim3 grid(ceil_div(N, GT), ceil_div(rows, GT));
     const Scales part = {s.a + m0, s.b, s.bias};
-    generic_kernel<Y><<<grid, G_THREADS, 0, stream>>>(A + size_t(m0) * K, B, out + size_t(m0) * N, rows, N, K, part);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(G_THREADS);
+    cfg.stream = stream;
+    // (the launch's own return code: the last error may be one of the caller's)
+    if (cudaLaunchKernelEx(&cfg, generic_kernel<Y>, A + size_t(m0) * K, B, out + size_t(m0) * N, rows, N, K, part) !=
+        cudaSuccess) {
+      cudaGetLastError();
+      return false;
+    }
     ++launch_counter();
     if (m0 > M - ROWS) break;  // m0 + ROWS would pass the int range
   }
   last_path() = PATH_GENERIC;
-  return cudaPeekAtLastError() == cudaSuccess;
+  return true;
 }
 
 // Clusters of `cluster` CTAs that the device holds at once.
@@ -1086,10 +1095,14 @@ struct DeviceSetup {
 static DeviceSetup setups[MAX_DEVICES];
 template <typename Y>
 static void configure_kernels() {
-  cudaFuncSetAttribute(stream_kernel<Y, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, S_SMEM_LIMIT);
-  cudaFuncSetAttribute(stream_kernel<Y, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, S_SMEM_LIMIT);
-  cudaFuncSetAttribute(pair_kernel<Y, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, P_SMEM_BYTES);
-  cudaFuncSetAttribute(pair_kernel<Y, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, P_SMEM_BYTES);
+  auto allow = [](auto* kernel, int smem_bytes) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes) != cudaSuccess)
+      cudaGetLastError();
+  };
+  allow(stream_kernel<Y, false>, S_SMEM_LIMIT);
+  allow(stream_kernel<Y, true>, S_SMEM_LIMIT);
+  allow(pair_kernel<Y, true>, P_SMEM_BYTES);
+  allow(pair_kernel<Y, false>, P_SMEM_BYTES);
 }
 static DeviceSetup& device_setup(DeviceCtx& ctx) {
   DeviceSetup& d = setups[ctx.device];
@@ -1107,7 +1120,6 @@ static DeviceSetup& device_setup(DeviceCtx& ctx) {
       }
     }
     d.pairs = max_clusters(pair_kernel<__half, true>, P_THREADS, P_SMEM_BYTES, 2);
-    cudaGetLastError();
     d.ready = true;
   }
   return d;
@@ -1277,11 +1289,7 @@ static int solve(const int8_t* A, const int8_t* B, Y* out, int M, int N, int K, 
       return 0;
     }
   }
-  if (!launch_generic(A, B, out, M, N, K, s, stream)) {
-    cudaGetLastError();
-    return -3;
-  }
-  return 0;
+  return launch_generic(A, B, out, M, N, K, s, stream) ? 0 : -3;
 }
 
 }  // namespace i8t
