@@ -89,3 +89,80 @@ def test_an_error_of_the_callers_is_left_alone(ops, K):
     finally:
         runtime.cudaGetLastError()
     assert torch.equal(out, want)
+
+
+# ------------------------------------------------------------------ several tiles per cluster
+# (M, N, K), path forced, path taken; on 148 SMs: R, CTAs of a cluster, clusters, tiles
+ROUNDS = [
+    ((1, 38976, 2576), 0, 2),     # 16, 3, 45, 153
+    ((16, 57344, 8192), 0, 2),    # 16, 3, 45, 224: a wide fused gate/up projection in decode
+    ((27, 38752, 3008), 0, 2),    # 32, 3, 45, 152
+    ((56, 38576, 3504), 0, 2),    # 64, 4, 33, 151
+    ((73, 19520, 7040), 0, 2),    # 128, 5, 26, 77
+    ((87, 19392, 6816), 0, 2),    # 128, 3, 45, 76
+    ((128, 57344, 8192), 0, 2),   # 128, 3, 45, 224
+    ((384, 4096, 14336), 0, 2),   # 128, 5, 26, 48: three rows of tiles
+    ((1, 38422, 1424), 0, 3),     # 16, 3, 45, 151, gathering from here on
+    ((8, 21730, 1514), 0, 3),     # 16, 3, 45, 85
+    ((64, 13220, 3113), 0, 3),    # 64, 5, 26, 52
+    ((128, 13220, 3113), 3, 3),   # 128, 5, 26, 52
+    ((128, 24020, 1483), 3, 3),   # 128, 4, 33, 94
+    ((200, 9988, 4453), 3, 3),    # 128, 3, 45, 80: two rows of tiles
+    ((16, 21728, 1536), 3, 3),    # 16, 3, 45, 85, aligned operands
+    ((64, 13216, 3120), 3, 3),    # 64, 5, 26, 52, aligned operands
+]
+
+
+@pytest.mark.parametrize("shape,force,path", ROUNDS)
+@pytest.mark.parametrize("out_type", [BF16, F32])
+def test_mm_several_tiles_per_cluster(ops, shape, force, path, out_type):
+    """A cluster that splits K and joins through its ring, tile after tile: the ring fills again only once
+    the partials of the tile before have been read.  Three calls in a row on different activations,
+    against 64 bits and, bit for bit, the SIMT kernel."""
+    from texo_b200 import _lib
+
+    M, N, K = shape
+    t = dtype(out_type)
+    A, B, sa, sb, bias = mm_inputs(M, N, K, M + N + K, full_range=True)
+    batches = [A, A.flip(0).contiguous(), A.flip(1).contiguous()]
+    ops.mm_int8_per_token(A[:1], B, sa[:1], sb)  # the device's set-up
+    lib = _lib.load()
+    lib.texo_mm_int8_per_token_force_path(force)
+    try:
+        got = [ops.mm_int8_per_token(a, B, sa, sb, bias, out_dtype=t) for a in batches]
+        assert lib.texo_mm_int8_per_token_last_path() == path
+        lib.texo_mm_int8_per_token_force_path(1)
+        simt = [ops.mm_int8_per_token(a, B, sa, sb, bias, out_dtype=t) for a in batches]
+        assert lib.texo_mm_int8_per_token_last_path() == 1
+    finally:
+        lib.texo_mm_int8_per_token_force_path(0)
+    for a, y, want in zip(batches, got, simt):
+        assert torch.equal(y, want)
+    want, bound = mm_expected(A, B, sa, sb, bias, t)
+    assert_within(got[0], want, bound)
+    assert ops.status() == 0
+
+
+def test_mm_several_tiles_per_cluster_on_two_streams_and_replayed(ops):
+    cases = [mm_inputs(16, 38976, 2576, 1), mm_inputs(8, 21730, 1514, 2)]
+    want = [ops.mm_int8_per_token(*c, out_dtype=torch.float32) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    results = [[], []]
+    for _ in range(10):
+        for case, stream, kept in zip(cases, streams, results):
+            with torch.cuda.stream(stream):
+                kept.append(ops.mm_int8_per_token(*case, out_dtype=torch.float32))
+    torch.cuda.synchronize()
+    for w, kept in zip(want, results):
+        assert all(torch.equal(w, y) for y in kept)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = [ops.mm_int8_per_token(*c, out_dtype=torch.float32) for c in cases]
+    for _ in range(3):
+        for o in outs:
+            o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(w, o) for w, o in zip(want, outs))
+    assert ops.status() == 0
