@@ -348,7 +348,10 @@ int texo_block_norm_solve(const void* x, const void* residual, const void* weigh
                           int x_type, int residual_type, int weights_f32, void* stream);
 /* The same with y quantised per token: scale [N] FP32, q [N,C] int8,
  *   scale = max(max_j |y|, 2^-100) / 127,   q = rint(y / scale)
- * (within [-127, 127]; both quotients rounded to FP32).  A row whose y holds a NaN or an infinity gets scale NaN and q = 0. */
+ * (within [-127, 127]).  scale is the quotient rounded to FP32.  rint takes y / scale rounded to FP32
+ * too, but from a value within 2^-46 of it, relative: exact ties are kept, and what lies that close to the
+ * middle between two FP32 values may round the other way (no y of 16 bits does).
+ * A row whose y holds a NaN or an infinity gets scale NaN and q = 0. */
 int texo_block_norm_quant_solve(const void* x, const void* residual, const void* weight,
                                 const void* post_weight, const void* gate, int8_t* q, float* scale,
                                 void* z, int N, int C, int gate_rows, int gate_per_channel, float eps,

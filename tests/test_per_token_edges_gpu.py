@@ -166,3 +166,73 @@ def test_mm_several_tiles_per_cluster_on_two_streams_and_replayed(ops):
         torch.cuda.synchronize()
         assert all(torch.equal(w, o) for w, o in zip(want, outs))
     assert ops.status() == 0
+
+
+# ------------------------------------------------------------------ the quotient y / scale
+def quotients(x):
+    """x / scale and its scale as IEEE divisions give them, and the quotient in 64 bits."""
+    top = x.float().abs().amax(dim=1).clamp_min(2.0 ** -100)
+    scale = top / torch.full_like(top, 127.0)  # (a division by a tensor; by a number it is a product)
+    return scale, x.float() / scale[:, None], x.double() / scale.double()[:, None]
+
+
+@pytest.mark.parametrize("x_type", [F16, BF16])
+@pytest.mark.parametrize("exponent", [-14, 0, 15, 100, 120])
+def test_quotients_of_16_bit_values_are_those_of_a_division(ops, x_type, exponent):
+    """Every row maximum of one binade against every value of the nine binades up to it (below, q = 0)."""
+    if x_type == F16 and exponent > 15:
+        pytest.skip("out of FP16's range")
+    bits = 10 if x_type == F16 else 7
+    steps = torch.arange(2 ** bits, device="cuda", dtype=torch.float64) / 2 ** bits + 1
+    tops = steps * 2.0 ** exponent
+    below = (steps[None] * 2.0 ** torch.arange(exponent - 8, exponent + 1, device="cuda", dtype=torch.float64)[:, None]).flatten()
+    values = torch.minimum(below[None], tops[:, None])
+    values = values * (1 - 2 * (torch.arange(values.shape[1], device="cuda") % 2))  # both signs
+    x = torch.cat([tops[:, None], values], dim=1).to(dtype(x_type))
+    q, s = ops.quant_per_token(x)
+    scale, quotient, _ = quotients(x)
+    assert torch.equal(s, scale)
+    assert torch.equal(q.float(), torch.round(quotient))
+
+
+@pytest.mark.parametrize("exponent", [0, -90, 105, 110, 127])
+def test_quotients_next_to_ties(ops, exponent):
+    """FP32 values up to three ulps around every tie, for a thousand row maxima: q is rint of the FP32 quotient
+    but where the true one lies within 2^-45 (twice the documented distance) of the middle between two
+    FP32 values, as one in 2^20 does, less than two of these 1.8 million.  Exact ties go to the even side."""
+    g = generator(exponent + 200)
+    rows = 1000
+    # below 2^128: the largest mantissas are left to the smaller exponents
+    tops = (1 + torch.rand(rows, generator=g, device="cuda", dtype=torch.float64) * 0.999).float() * 2.0 ** exponent
+    scale = tops / torch.full_like(tops, 127.0)
+    halves = torch.arange(-126, 126, device="cuda", dtype=torch.float64) + 0.5
+    near = (scale.double()[:, None] * halves).float()
+    ulps = torch.arange(-3, 4, device="cuda", dtype=torch.int32)
+    near = (near.view(torch.int32)[:, :, None] + ulps).view(torch.float32).reshape(rows, -1)
+    x = torch.cat([tops[:, None], near], dim=1)
+    assert bool(torch.isfinite(x).all()) and bool((x.abs() <= tops[:, None]).all())
+    q, s = ops.quant_per_token(x)
+    scale, quotient, exact = quotients(x)
+    assert torch.equal(s, scale)
+    other = q.float() != torch.round(quotient)
+    up = torch.nextafter(quotient, torch.full_like(quotient, float("inf"))).double()
+    down = torch.nextafter(quotient, torch.full_like(quotient, float("-inf"))).double()
+    to_middle = torch.minimum((exact - (quotient.double() + up) / 2).abs(), (exact - (quotient.double() + down) / 2).abs())
+    assert not bool((other & (to_middle > exact.abs() * 2.0 ** -45)).any())
+    assert int(other.sum()) <= 4
+    tie = exact == torch.floor(exact) + 0.5
+    assert torch.equal(q[tie].double(), torch.round(exact[tie]))
+
+
+@pytest.mark.parametrize("C", [64, 1001, 8192, 16385])
+@pytest.mark.parametrize("size", [1.0, 2.0 ** 100, 2.0 ** 115])
+def test_quantised_norm_is_the_quantiser_of_the_norm(ops, C, size):
+    """In FP32 the norm's y is what its quantised form quantises, huge rows included."""
+    g = generator(C)
+    x, r = (torch.randn(7, C, generator=g, device="cuda") for _ in range(2))
+    w = (1 + 0.2 * torch.randn(C, generator=g, device="cuda")) * size
+    y, _ = ops.block_norm(x, r, w, 1e-5)
+    q, s, _ = ops.block_norm_quant_per_token(x, r, w, 1e-5)
+    q1, s1 = ops.quant_per_token(y)
+    assert torch.equal(q, q1) and torch.equal(s, s1)
+    assert bool((s > size / 127).all())

@@ -114,6 +114,7 @@ __device__ __forceinline__ void finish(const Args& a, int n, X* y, int8_t* q, co
     amax = row::row_max(amax, max_scratch, s.t, warps);
     const row::TokenScale scale = row::token_scale(amax);
     if (s.t == 0) a.scale[n] = scale.scale;
+    row::shrink_huge(v, scale);
 #pragma unroll
     for (int i = 0; i < UNITS; ++i) s.store_quantised(q, i, v[i], scale);
   }

@@ -65,8 +65,9 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {  // 16-byte 
 }
 
 // The per-token quantiser: scale = max(amax, 2^-100) / 127, q = rint(y / scale), both quotients
-// rounded to FP32 first: values half way between two multiples of the scale are common where y
-// has few bits, and a product with a rounded 127 / amax would take them off the tie.
+// rounded to FP32 first (y / scale from a value within 2^-46 of it, see below): values half way between two
+// multiples of the scale are common where y has few bits, and a product with a rounded 127 / amax
+// would take them off the tie.
 // The floor keeps scale and reciprocal finite and non-zero for every row (a row of zeros gets
 // q = 0).  A row that holds a NaN or an infinity has no scale that stands for it: its scale is
 // NaN and its q all zero, so that whatever the row is multiplied into shows it.
@@ -80,8 +81,13 @@ struct TokenScale {
 // processor", 1990).  scale: q0 = a * RN(1/127) is within two ulps of a/127; q1 = q0 + (a - 127 q0) *
 // RN(1/127) within one; the same step from there rounds correctly.  y / scale: one Newton step takes
 // the approximate reciprocal r to hi = r + (1 - scale r) r, within half an ulp and a little; lo = (1 - scale hi)
-// hi is the rest, and hi + lo is within 2^-47 of 1/scale.  A few instructions that every thread can
-// afford, where divisions take an eighth of a short row's time.
+// hi is the rest.  hi + lo is within 2^-47 of 1/scale, and y hi + RN(y lo) within 2^-46 of the quotient, so
+// that it rounds like the quotient unless that lies so close to the middle between two FP32 values.  (The
+// correction step once more instead of lo would round correctly and costs 3% of a plain quantiser's time.)
+// From scale = 2^102 on lo would be subnormal and lose bits, so there hi, lo and y are those of a row
+// 2^64 times smaller.  A few instructions that every thread can afford, where divisions take an eighth of
+// a short row's time.
+constexpr float HUGE_SCALE = 0x1p100f, HUGE_TOP = 0x1p106f /*below which no scale is huge*/, SHRINK = 0x1p-64f;
 __device__ __forceinline__ TokenScale token_scale(float amax) {
   TokenScale s;
   if (__float_as_uint(amax) >= 0x7f800000u) {
@@ -95,15 +101,17 @@ __device__ __forceinline__ TokenScale token_scale(float amax) {
   q = __fmaf_rn(__fmaf_rn(-127.f, q, top), BY_127, q);
   s.scale = __fmaf_rn(__fmaf_rn(-127.f, q, top), BY_127, q);
   float r;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(s.scale));
-  s.hi = __fmaf_rn(__fmaf_rn(-s.scale, r, 1.f), r, r);
-  s.lo = __fmul_rn(__fmaf_rn(-s.scale, s.hi, 1.f), s.hi);
+  const float divisor = s.scale >= HUGE_SCALE ? s.scale * SHRINK : s.scale;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(divisor));
+  s.hi = __fmaf_rn(__fmaf_rn(-divisor, r, 1.f), r, r);
+  s.lo = __fmul_rn(__fmaf_rn(-divisor, s.hi, 1.f), s.hi);
   return s;
 }
 // Adding this (1.5 * 2^23) to |t| < 2^22 rounds t to the nearest integer, whose low byte is then the
 // sum's (a conversion instruction runs at an eighth of the rate).
 constexpr float ROUND_TO_INTEGER = 12582912.f;
 __device__ __forceinline__ int8_t quantise(float v, const TokenScale& s) {
+  if (s.scale >= HUGE_SCALE) v *= SHRINK;
   const float quotient = __fmaf_rn(v, s.hi, __fmul_rn(v, s.lo));
   return s.hi == 0.f ? int8_t(0) : int8_t(uint8_t(__float_as_uint(__fadd_rn(quotient, ROUND_TO_INTEGER))));
 }
@@ -143,6 +151,15 @@ __device__ __forceinline__ void mul8(float (&v)[8], const A& a, const B& b) {
         : "=l"(d)
         : "l"(pair_of(lane8(a, j), lane8(a, j + 1))), "l"(pair_of(lane8(b, j), lane8(b, j + 1))));
     from_pair(d, v[j], v[j + 1]);
+  }
+}
+
+// A thread's values as the scale's hi and lo expect them (a branch that no ordinary row takes).
+template <int UNITS>
+__device__ __forceinline__ void shrink_huge(float (&v)[UNITS][8], const TokenScale& s) {
+  if (s.scale >= HUGE_SCALE) {
+#pragma unroll
+    for (int i = 0; i < UNITS; ++i) mul8(v[i], v[i], float(SHRINK));
   }
 }
 
@@ -199,7 +216,7 @@ struct Spread {
     }
   }
 
-  // The same for v quantised (ALIGNED: rows start at 8-byte boundaries).
+  // The same for v (after shrink_huge) quantised (ALIGNED: rows start at 8-byte boundaries).
   __device__ __forceinline__ void store_quantised(int8_t* row, int i, const float (&v)[8], const TokenScale& scale) const {
     uint32_t r[8] = {};
     if (scale.hi != 0.f) {
