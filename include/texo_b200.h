@@ -364,8 +364,8 @@ int texo_quant_per_token_solve(const void* x, int8_t* q, float* scale, int N, in
 /* The same behind the SwiGLU product: y[n,j] = silu(gate[n,j]) * up[n,j], q [N,F].  gate_up has
  * 2F values per row: gate j and up j at 2j and 2j+1 if interleaved (the column order of
  * texo_mm_int8_swiglu_solve), else at j and F+j.  y is within (9 + 1.23 |gate|) * 2^-24 of its value
- * (gates below -80: 11 * 2^-24 and 2^-115), also where exp(-gate) or gate * up would overflow; rows
- * with a gate below -87 or a product that overflows are read twice more. */
+ * (gates below -87: 11 * 2^-24 and 2^-115), also where exp(-gate) or gate * up would overflow; rows
+ * with a gate below -87 or a |y| beyond 2^106 are read twice more. */
 int texo_swiglu_quant_per_token_solve(const void* gate_up, int8_t* q, float* scale, int N, int F,
                                       long long row_stride, int interleaved, int x_type,
                                       void* stream);

@@ -236,3 +236,38 @@ def test_quantised_norm_is_the_quantiser_of_the_norm(ops, C, size):
     q1, s1 = ops.quant_per_token(y)
     assert torch.equal(q, q1) and torch.equal(s, s1)
     assert bool((s > size / 127).all())
+
+
+@pytest.mark.parametrize("F", [1, 7, 65, 1025, 8191])
+@pytest.mark.parametrize("x_type", [F16, BF16, F32])
+@pytest.mark.parametrize("interleaved", [True, False])
+def test_swiglu_rows_do_not_depend_on_what_lies_behind_them(ops, F, x_type, interleaved):
+    """Rows of ordinary gates (down to -86.5) whose neighbours in memory begin and end with far ones: the
+    same bits as each row alone."""
+    g = generator(F)
+    rows = 64
+    gate = torch.rand(rows, F, generator=g, device="cuda") * -5.5 - 81
+    up = (torch.rand(rows, F, generator=g, device="cuda") + 0.5) * (6e4 if x_type == F16 else 1e30)
+    gate[1::2] = -1e4
+    up[1::2] = -6e4
+    gate, up = gate.to(dtype(x_type)), up.to(dtype(x_type))
+    x = torch.stack([gate, up], dim=2).reshape(rows, 2 * F) if interleaved else torch.cat([gate, up], dim=1)
+    q, s = ops.swiglu_quant_per_token(x.contiguous(), interleaved=interleaved)
+    for r in range(0, rows, 2):
+        q1, s1 = ops.swiglu_quant_per_token(x[r:r + 1].contiguous(), interleaved=interleaved)
+        # (in FP16 some rows hold an infinity: NaN scales, compared by their bits)
+        assert torch.equal(s1.view(torch.int32)[0], s.view(torch.int32)[r]) and torch.equal(q1[0], q[r])
+
+
+@pytest.mark.parametrize("F", [64, 1024, 1025, 8191, 28672])
+@pytest.mark.parametrize("x_type", [F16, BF16, F32])
+@pytest.mark.parametrize("interleaved", [True, False])
+def test_swiglu_far_gates_in_large_batches(ops, F, x_type, interleaved):
+    """Batches whose rows are not all at work at once lay a row out differently (four groups per thread)."""
+    gate, up = far_rows(F, x_type, F)
+    x = torch.stack([gate, up], dim=2).reshape(8, 2 * F) if interleaved else torch.cat([gate, up], dim=1)
+    q, s = ops.swiglu_quant_per_token(x.contiguous(), interleaved=interleaved)
+    copies = 160
+    qs, ss = ops.swiglu_quant_per_token(x.repeat(copies, 1), interleaved=interleaved)
+    assert torch.equal(ss.view(copies, 8), s.expand(copies, 8))
+    assert torch.equal(qs.view(copies, 8, F), q.expand(copies, 8, F))

@@ -62,11 +62,12 @@ __device__ __forceinline__ void swiglu8(const float (&gate)[8], const float (&up
   row::mul8(product, gate, up);
   row::mul8(y, t, product);
 }
-// For any finite gate and up.  Below -80, 1 + e^-gate is e^-gate, and y = (gate h) (h up) with h =
-// e^(gate / 2): no factor leaves the range unless y does (h is subnormal below -174, where |y| < 2^-115
-// whatever up is, a hundredth of the smallest scale).  Where the product overflows the quotient comes first.
+// For any finite gate and up, and the same bits where `swiglu` is good.  Below -87, 1 + e^-gate is e^-gate, and
+// y = (gate h) (h up) with h = e^(gate / 2): no factor leaves the range unless y does (h is subnormal
+// below -174, where |y| < 2^-115 whatever up is, a hundredth of the smallest scale).  Where the product
+// overflows the quotient comes first.
 __device__ __forceinline__ float careful_swiglu(float gate, float up) {
-  if (gate < -80.f) {
+  if (gate < LOWEST_GATE) {
     const float h = expf(0.5f * gate);
     return (gate * h) * (h * up);
   }
@@ -103,7 +104,8 @@ __device__ __forceinline__ void load_y(const X* x, const row::Spread<row::ALIGNE
     swiglu_pairs(lo, hi, y, lowest);
   }
 }
-// The same of a staged row: `first` holds x (or the gates, `second` the ups).
+// The same of a staged row: `first` holds x (or the gates, `second` the ups).  What lies past the row's end is
+// arbitrary; it is masked before anything is computed from it.
 template <typename X, int FORM>
 __device__ __forceinline__ void read_y(uint32_t first, unsigned offset, uint32_t second, unsigned second_offset,
                                        const row::Spread<row::STAGED>& s, int i, float (&y)[8], float& lowest) {
@@ -116,16 +118,25 @@ __device__ __forceinline__ void read_y(uint32_t first, unsigned offset, uint32_t
     float lo[8], hi[8];
     row::read_staged<X>(first, offset, 2 * s.at(i, 0), lo);
     row::read_staged<X>(first, offset, 2 * s.at(i, 0) + 8, hi);
+    const row::Spread<row::STAGED> wide = {0, 1, 2 * s.C};
+    wide.mask(s.at(i, 0) / 4, lo);
+    wide.mask(s.at(i, 0) / 4 + 1, hi);
     swiglu_pairs(lo, hi, y, lowest);
   } else {
     row::read_staged<X>(first, offset, s.at(i, 0), y);
     if (FORM == SWIGLU_HALVES) {
       float u[8];
       row::read_staged<X>(second, second_offset, s.at(i, 0), u);
+      if (s.at(i, 8) > s.C) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (s.at(i, j) >= s.C) y[j] = u[j] = 0.f;
+      }
       swiglu8(y, u, y, lowest);
+    } else {
+      s.mask(i, y);
     }
   }
-  s.mask(i, y);  // (what lies past the row's end is arbitrary)
 }
 
 // Threads of a block at most, and such blocks that an SM has to hold for their latencies to overlap.
