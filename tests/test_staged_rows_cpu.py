@@ -20,6 +20,7 @@ static long long extent(int C, int size, bool pairs) {
   const long long last = (C - 1) / 8 * 8;                // first value of the last group of eight outputs
   const long long granules = size * 2 / 4 + 1;           // that read_staged loads for eight values
   covers((pairs ? 2 * last + 8 : last) * size + granules * 16);
+  covers(15 + (last + 8) * size * (pairs ? 2 : 1));      // clear_staged: to the end of the last group
   if (!pairs) covers((last + 8) * size);                 // store: whole groups
   covers(last + 8);                                      // store_quantised
   covers((long long)C / 16 * 16 + 16);                   // send_row of q: one granule more than it sends

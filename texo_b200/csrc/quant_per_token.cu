@@ -62,6 +62,25 @@ __device__ __forceinline__ void swiglu8(const float (&gate)[8], const float (&up
   row::mul8(product, gate, up);
   row::mul8(y, t, product);
 }
+// The same, two values after two: the registers of gate and up are free sooner, which rows in halves,
+// whose operands come from two places, are short of (4096 x 14336 FP16 60 -> 54.8 us; pairs of 28672
+// BF16 take 125 us so instead of 120).
+__device__ __forceinline__ void swiglu8_by_twos(const float (&gate)[8], const float (&up)[8], float (&y)[8], float& lowest) {
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    asm("min.f32 %0, %0, %1, %2;" : "+f"(lowest) : "f"(gate[j]), "f"(gate[j + 1]));
+    const unsigned long long g = row::pair_of(gate[j], gate[j + 1]);
+    const unsigned long long product = row::mul2(g, row::pair_of(up[j], up[j + 1]));
+    float a, b;
+    row::from_pair(row::mul2(g, row::pair_of(-LOG2_E, -LOG2_E)), a, b);
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(b));
+    row::from_pair(row::fma2(row::pair_of(a, b), row::pair_of(1.f, 1.f), row::pair_of(1.f, 1.f)), a, b);
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(a));
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(b));
+    row::from_pair(row::mul2(row::pair_of(a, b), product), y[j], y[j + 1]);
+  }
+}
 // For any finite gate and up, and the same bits where `swiglu` is good.  Below -87, 1 + e^-gate is e^-gate, and
 // y = (gate h) (h up) with h = e^(gate / 2): no factor leaves the range unless y does (h is subnormal
 // below -174, where |y| < 2^-115 whatever up is, a hundredth of the smallest scale).  Where the product
@@ -93,7 +112,7 @@ __device__ __forceinline__ void load_y(const X* x, const row::Spread<row::ALIGNE
     float g[8], u[8];
     s.template load<true>(x, i, g);
     s.template load<true>(x + s.C, i, u);
-    swiglu8(g, u, y, lowest);
+    swiglu8_by_twos(g, u, y, lowest);
   } else {
     // the sixteen inputs of eight outputs: two groups of a row of 2 C values
     const row::Spread<row::ALIGNED> wide = {0, 1, 2 * s.C};
@@ -105,7 +124,8 @@ __device__ __forceinline__ void load_y(const X* x, const row::Spread<row::ALIGNE
   }
 }
 // The same of a staged row: `first` holds x (or the gates, `second` the ups).  What lies past the row's end is
-// arbitrary; it is masked before anything is computed from it.
+// arbitrary; in rows of SwiGLU operands, where it must not count as a gate, the thread that reads it makes
+// it zero first (nobody else uses it).
 template <typename X, int FORM>
 __device__ __forceinline__ void read_y(uint32_t first, unsigned offset, uint32_t second, unsigned second_offset,
                                        const row::Spread<row::STAGED>& s, int i, float (&y)[8], float& lowest) {
@@ -114,40 +134,35 @@ __device__ __forceinline__ void read_y(uint32_t first, unsigned offset, uint32_t
     for (int j = 0; j < 8; ++j) y[j] = 0.f;
     return;
   }
+  if (FORM == PLAIN) {
+    row::read_staged<X>(first, offset, s.at(i, 0), y);
+    s.mask(i, y);
+    return;
+  }
+  if (s.at(i, 8) > s.C) {
+    constexpr int WIDTH = FORM == SWIGLU_INTERLEAVED ? 2 : 1;
+    row::clear_staged<X>(first, offset, WIDTH * s.C, WIDTH * s.at(i, 8));
+    if (FORM == SWIGLU_HALVES) row::clear_staged<X>(second, second_offset, s.C, s.at(i, 8));
+  }
   if (FORM == SWIGLU_INTERLEAVED) {
     float lo[8], hi[8];
     row::read_staged<X>(first, offset, 2 * s.at(i, 0), lo);
     row::read_staged<X>(first, offset, 2 * s.at(i, 0) + 8, hi);
-    const row::Spread<row::STAGED> wide = {0, 1, 2 * s.C};
-    wide.mask(s.at(i, 0) / 4, lo);
-    wide.mask(s.at(i, 0) / 4 + 1, hi);
     swiglu_pairs(lo, hi, y, lowest);
   } else {
-    row::read_staged<X>(first, offset, s.at(i, 0), y);
-    if (FORM == SWIGLU_HALVES) {
-      float u[8];
-      row::read_staged<X>(second, second_offset, s.at(i, 0), u);
-      if (s.at(i, 8) > s.C) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (s.at(i, j) >= s.C) y[j] = u[j] = 0.f;
-      }
-      swiglu8(y, u, y, lowest);
-    } else {
-      s.mask(i, y);
-    }
+    float g[8], u[8];
+    row::read_staged<X>(first, offset, s.at(i, 0), g);
+    row::read_staged<X>(second, second_offset, s.at(i, 0), u);
+    swiglu8_by_twos(g, u, y, lowest);
   }
 }
 
-// Threads of a block at most, and such blocks that an SM has to hold for their latencies to overlap.
-// Two blocks of 576 leave 56 registers instead of 64, hence three blocks of 352 instead of two: rows
-// of 11008 30.6 -> 24.7 us, as halves 48.5 -> 41.9.  Interleaved pairs want the 64 (4096 x 28672: 120
-// us against 142).
+// Threads of a block at most.  Two blocks of 576 leave 56 registers instead of 64, hence three blocks of
+// 352 instead of two: rows of 11008 30.6 -> 24.7 us, as halves 48.5 -> 41.9, staged pairs of 4000 x 11007
+// 69.7 -> 58.2.  Interleaved pairs in aligned rows want the 64 (4096 x 28672: 120 us against 142).
+constexpr int SHORT = 576;
 __host__ __device__ constexpr int block_limit(int form, row::Layout layout, int units) {
-  return layout == row::STAGED || units < 4 ? 1024 : form == SWIGLU_INTERLEAVED ? 512 : 576;
-}
-__host__ __device__ constexpr int blocks_per_sm(row::Layout layout, int units) {
-  return layout == row::STAGED || units == 1 ? 1 : 2;
+  return layout == row::STAGED || units < 4 ? 1024 : form == SWIGLU_INTERLEAVED ? 512 : SHORT;
 }
 
 // A row whose y is computed twice, value by value, by `threads` threads in `blocks` blocks.
@@ -180,8 +195,8 @@ __device__ __forceinline__ void careful_row(const Args& a, int blocks, unsigned*
 }
 
 // A block, a warp or (blocks > 1) a cluster per row.  blockDim = (threads, rows of the block).
-template <typename X, int FORM, row::Layout L, int UNITS>
-__global__ void __launch_bounds__(block_limit(FORM, L, UNITS), blocks_per_sm(L, UNITS)) row_kernel(const Args a, int blocks) {
+template <typename X, int FORM, row::Layout L, int UNITS, int LIMIT = block_limit(FORM, L, UNITS)>
+__global__ void __launch_bounds__(LIMIT, LIMIT <= SHORT ? 2 : 1) row_kernel(const Args a, int blocks) {
   __shared__ unsigned scratch[2][row::MAX_WARPS], maxima[2][row::MAX_CLUSTER];
   grid_dependency_trigger();
   row::cluster_started(blocks);
@@ -259,6 +274,8 @@ static bool launch(const Args& a, cudaStream_t stream) {
     if (!row::at_once(r, a.N, 1536)) r = row::plan_row(a.C, 4, block_limit(FORM, row::STAGED, 4), 1, false);
     if (r.units == 0 || room > row::SMEM_LIMIT) return launch_long();
     auto rows = [&](auto* kernel) { return row::launch_staged(kernel, unsigned(a.N), dim3(r.threads), room, stream, a, 1); };
+    if constexpr (FORM != PLAIN)
+      if (r.units == 4 && r.threads <= SHORT) return rows(row_kernel<X, FORM, row::STAGED, 4, SHORT>);
     return r.units == 1 ? rows(row_kernel<X, FORM, row::STAGED, 1>) : rows(row_kernel<X, FORM, row::STAGED, 4>);
   }
   // 8192 x 8192 BF16: 60 / 41 / 35 us for one / two / four groups per thread; 4096 x 28672

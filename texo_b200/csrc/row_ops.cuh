@@ -126,32 +126,33 @@ __device__ __forceinline__ unsigned long long pair_of(float a, float b) {
 __device__ __forceinline__ void from_pair(unsigned long long p, float& a, float& b) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
 }
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
+  unsigned long long d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 // v = a * b + c, each of them eight values or one.
 __device__ __forceinline__ float lane8(const float (&v)[8], int j) { return v[j]; }
 __device__ __forceinline__ float lane8(float v, int) { return v; }
 template <typename A, typename B, typename C>
 __device__ __forceinline__ void fma8(float (&v)[8], const A& a, const B& b, const C& c) {
 #pragma unroll
-  for (int j = 0; j < 8; j += 2) {
-    unsigned long long d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;"
-        : "=l"(d)
-        : "l"(pair_of(lane8(a, j), lane8(a, j + 1))), "l"(pair_of(lane8(b, j), lane8(b, j + 1))),
-          "l"(pair_of(lane8(c, j), lane8(c, j + 1))));
-    from_pair(d, v[j], v[j + 1]);
-  }
+  for (int j = 0; j < 8; j += 2)
+    from_pair(fma2(pair_of(lane8(a, j), lane8(a, j + 1)), pair_of(lane8(b, j), lane8(b, j + 1)),
+                   pair_of(lane8(c, j), lane8(c, j + 1))),
+              v[j], v[j + 1]);
 }
 // v = a * b.
 template <typename A, typename B>
 __device__ __forceinline__ void mul8(float (&v)[8], const A& a, const B& b) {
 #pragma unroll
-  for (int j = 0; j < 8; j += 2) {
-    unsigned long long d;
-    asm("mul.rn.f32x2 %0, %1, %2;"
-        : "=l"(d)
-        : "l"(pair_of(lane8(a, j), lane8(a, j + 1))), "l"(pair_of(lane8(b, j), lane8(b, j + 1))));
-    from_pair(d, v[j], v[j + 1]);
-  }
+  for (int j = 0; j < 8; j += 2)
+    from_pair(mul2(pair_of(lane8(a, j), lane8(a, j + 1)), pair_of(lane8(b, j), lane8(b, j + 1))), v[j], v[j + 1]);
 }
 
 // A thread's values as the scale's hi and lo expect them (a branch that no ordinary row takes).
@@ -311,6 +312,16 @@ __device__ __forceinline__ void read_staged(uint32_t row, unsigned offset, int i
       v[2 * k] = p.x;
       v[2 * k + 1] = p.y;
     }
+  }
+}
+
+// Makes the values from `begin` to `end` of a fetched row zero.
+template <typename T>
+__device__ __forceinline__ void clear_staged(uint32_t row, unsigned offset, int begin, int end) {
+  for (int i = begin; i < end; ++i) {
+    const uint32_t at = row + offset + i * int(sizeof(T));
+    if (sizeof(T) == 4) sts32(at, 0u);
+    else sts16(at, 0);
   }
 }
 
