@@ -186,7 +186,8 @@ __device__ __forceinline__ void row_in_passes(const Args& a, long long n, int t,
 }
 // Once more, for a row of SwiGLU products with a far gate, a huge value or one that is not finite.  The
 // row's number comes from the special registers again, which keeps it and the row's addresses out of the registers
-// until here (4096 x 28672 BF16 pairs 119.7 us, handed over 126.6).
+// until here (4096 x 28672 BF16 pairs 119.7 us, handed over 126.6).  Such a row costs five to seven others; in
+// vectors it costs three, but then the others pay 14% (in line) or halves 10% (as a call).
 template <typename X, int FORM>
 __device__ __forceinline__ void careful_row(const Args& a, int blocks, unsigned* scratch, unsigned* maxima) {
   row::cluster_started(blocks);

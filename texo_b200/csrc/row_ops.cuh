@@ -2,12 +2,13 @@
 // element types, layouts of a row over threads, reductions over a row, the per-token quantiser.
 //
 // These kernels read each byte once and write each byte once, so HBM bounds them; what keeps a
-// kernel from that bound is its instructions (a row of 16-bit values is ten to twenty per value)
-// and its latencies: loads, one to three reductions and stores follow one another within a
-// row.  The first is met by packed arithmetic, the second by many small blocks: one row per
-// block, 512 threads or fewer, as many blocks as an SM holds.  A persistent form (two to six
-// blocks per SM, rows arriving through a ring of bulk copies one or more rows ahead) hid the
-// loads but not the rest, and measured 89 us where this form takes 60 (4096 x 8192 BF16, both
+// kernel from that bound is its instructions (a row of 16-bit values is ten to thirty per value, a staged
+// one up to twice that) and above all its latencies: loads, one to three reductions and stores follow one
+// another within a row (2.2 to 2.8 instructions per clock and SM of four, with a third to a half of the warps an
+// SM holds).  The first is met by packed arithmetic, the second by many blocks: one row per block of up
+// to 1024 threads, as few as the groups per thread allow, and as many blocks as an SM holds.  A persistent
+// form (two to six blocks per SM, rows arriving through a ring of bulk copies one or more rows ahead)
+// hid the loads but not the rest, and measured 89 us where this form takes 60 (4096 x 8192 BF16, both
 // norms, gate, quantised).
 #pragma once
 #include <algorithm>
@@ -415,7 +416,8 @@ inline RowPlan plan_row(int C, int units, int most_threads, int most_blocks, boo
   p.rows_per_block = p.threads == 32 && p.cluster == 1 && aligned_rows ? 4 : 1;
   return p;
 }
-// Whether all rows are in work at once, on 148 SMs that hold `threads_per_sm` threads each.  Until
+// Whether all rows are in work at once, on the 148 SMs of a whole B200 (on a part of one the rule
+// sets in later, which costs time but no correctness) that hold `threads_per_sm` threads each.  Until
 // then the shortest way through a row wins, one group of eight per thread; after that more groups
 // per thread do, which spread a thread's fixed work over more values.
 inline bool at_once(const RowPlan& p, long long N, int threads_per_sm) {
