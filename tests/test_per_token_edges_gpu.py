@@ -1,10 +1,14 @@
 """GPU tests of the dynamic-quantisation operators at the ends of their ranges: values, sizes,
 errors of other calls, and the paths of the product that only large problems take.  Helpers and the
 counting of roundings are those of test_per_token_gpu.py."""
+import os
+import subprocess
+import sys
+
 import pytest
 
-from tests.test_per_token_gpu import (BF16, F16, F32, U, check_quantised, dtype, generator, mm_expected, mm_inputs,
-                                      assert_within, ops)  # noqa: F401  (ops is a fixture)
+from tests.test_per_token_gpu import (BF16, F16, F32, U, assert_within, check_quantised, dtype, generator, half_step,
+                                      mm_expected, mm_inputs, norm_expected, norm_inputs, ops)  # noqa: F401  (ops is a fixture)
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -271,3 +275,57 @@ def test_swiglu_far_gates_in_large_batches(ops, F, x_type, interleaved):
     qs, ss = ops.swiglu_quant_per_token(x.repeat(copies, 1), interleaved=interleaved)
     assert torch.equal(ss.view(copies, 8), s.expand(copies, 8))
     assert torch.equal(qs.view(copies, 8, F), q.expand(copies, 8, F))
+
+
+# ------------------------------------------------------------------ rooms about 48 KiB
+@pytest.mark.parametrize("C", range(24331, 24600, 42))
+def test_staged_rows_about_48_kib(ops, C):
+    """A block's staged rows and its own few words together may pass the 48 KiB that a kernel has without asking
+    where the rows alone do not.  C: FP16 values whose granules are 192 bytes below that to a little above."""
+    g = generator(C)
+    x = torch.randn(3, C, generator=g, device="cuda")
+    zero = torch.zeros((), dtype=torch.float64, device="cuda")
+    for part, call in ((x[:, :C].half(), ops.quant_per_token), (x[:, :C // 2], ops.quant_per_token)):
+        part = part[:, :part.shape[1] - (part.shape[1] % 8 == 0)].contiguous()
+        q, s = call(part)
+        check_quantised(q, s, part.double(), zero.expand(part.shape))
+    for dt, width in ((torch.float16, C // 2), (torch.float32, C // 4)):
+        F = width - (width % 8 == 0)
+        gu = torch.randn(3, 2 * F, generator=g, device="cuda").to(dt)
+        for interleaved in (True, False):
+            gate, up = (gu[:, 0::2], gu[:, 1::2]) if interleaved else (gu[:, :F], gu[:, F:])
+            gate, up = gate.double(), up.double()
+            y = gate * torch.sigmoid(gate) * up
+            q, s = ops.swiglu_quant_per_token(gu, interleaved=interleaved)
+            check_quantised(q, s, y, y.abs() * (12 + 1.24 * gate.abs()) * U + 2.0 ** -114)
+    for types, width in (((F16, F16, F16), C // 2), ((F16, F32, F32), C // 3), ((F32, F32, F32), C // 4)):
+        c = width - (width % 8 == 0)
+        x2, r, w, p, gt = norm_inputs(3, c, *types, "channel", C)
+        y64, dy, z64, dz = norm_expected(x2, r, w, p, gt, 1e-5, 1.0)
+        y, z = ops.block_norm(x2, r, w, 1e-5, post_weight=p, gate=gt)
+        assert_within(z, z64, dz + half_step(z64, z.dtype) * 1.01)
+        assert_within(y, y64, dy + half_step(y64, y.dtype) * 1.01)
+        q, s, _ = ops.block_norm_quant_per_token(x2, r, w, 1e-5, post_weight=p, gate=gt)
+        check_quantised(q, s, y64, dy)
+
+
+def test_the_first_call_about_48_kib(ops):
+    """The same in a process that has made no larger call before: a kernel keeps the room that it was once given."""
+    script = """
+import torch
+from texo_b200 import ops
+x = torch.randn(3, 24499, device="cuda")
+h = x.half()
+ops.quant_per_token(h), ops.quant_per_token(x[:, :12249].contiguous())
+for gu in (h[:, :24498].contiguous(), x[:, :12246].contiguous()):
+    for interleaved in (True, False):
+        ops.swiglu_quant_per_token(gu, interleaved=interleaved)
+for a, b in ((h[:, :12249], h[:, :12249]), (h[:, :8166], x[:, :8166]), (x[:, :6123], x[:, :6123])):
+    a, b = a.contiguous(), b.contiguous()
+    ops.block_norm(a, b, a[0].contiguous(), 1e-5), ops.block_norm_quant_per_token(a, b, a[0].contiguous(), 1e-5)
+torch.cuda.synchronize()
+print("ran")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", script], cwd=root, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "ran" in run.stdout, run.stderr

@@ -423,13 +423,14 @@ inline RowPlan plan_row(int C, int units, int most_threads, int most_blocks, boo
 inline bool at_once(const RowPlan& p, long long N, int threads_per_sm) {
   return p.units > 0 && N * p.cluster <= 148LL * (threads_per_sm / p.threads);
 }
-constexpr int SMEM_LIMIT = 232448 - 2048;  // (the kernels' own few words are static)
+constexpr int STATIC_ROOM = 2048;  // what the kernels' own few words take at most
+constexpr int SMEM_LIMIT = 232448 - STATIC_ROOM;
 // Launches a kernel on staged rows; the attribute is set before every launch that needs it, which
 // costs less than keeping track of devices and kernels.
 template <typename... Params, typename... Args>
 static bool launch_staged(void (*kernel)(Params...), unsigned grid, dim3 block, int bytes, cudaStream_t stream,
                           Args... args) {
-  if (bytes > 48 * 1024 &&
+  if (bytes > 48 * 1024 - STATIC_ROOM &&  // both together may be 48 KiB without the attribute
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT) != cudaSuccess) {
     cudaGetLastError();
     return false;
