@@ -2,6 +2,7 @@
 errors of other calls, and the paths of the product that only large problems take.  Helpers and the
 counting of roundings are those of test_per_token_gpu.py."""
 import os
+import random
 import subprocess
 import sys
 
@@ -329,3 +330,89 @@ print("ran")
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     run = subprocess.run([sys.executable, "-c", script], cwd=root, capture_output=True, text=True, timeout=300)
     assert run.returncode == 0 and "ran" in run.stdout, run.stderr
+
+
+# ------------------------------------------------------------------ random sizes, strides and addresses
+def spread(rng, lo, hi):
+    """An integer of [lo, hi], spread over its logarithm."""
+    return min(hi, max(lo, int(round(lo * (hi / lo) ** rng.random()))))
+
+
+def placed(x, by):
+    """A copy of x `by` elements into a larger buffer."""
+    base = torch.zeros(x.numel() + by, dtype=x.dtype, device="cuda")
+    base[by:] = x.reshape(-1)
+    return base[by:].view(x.shape)
+
+
+class Guarded:
+    """An output inside a larger buffer, 0 to 8 elements off a 16-byte boundary."""
+
+    def __init__(self, rng, rows, columns, t):
+        self.count = rows * columns
+        self.start = 32 + rng.choice([0, 0, 1, 3, 8])
+        self.base = torch.full((self.start + self.count + 32,), 77, dtype=t, device="cuda")
+        self.out = self.base[self.start:self.start + self.count].view(rows, columns)
+
+    def check(self):
+        assert bool((self.base[:self.start] == 77).all()) and bool((self.base[self.start + self.count:] == 77).all())
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_random_products(ops, seed):
+    rng = random.Random(seed)
+    for i in range(150):
+        M, N, K = spread(rng, 1, 900), spread(rng, 1, 6000), spread(rng, 1, 6000)
+        if rng.random() < 0.5:
+            N, K = (N + 15) // 16 * 16, (K + 15) // 16 * 16
+        A, B, sa, sb, bias = mm_inputs(M, N, K, 1000 * seed + i, full_range=True)
+        A, B = (placed(v, rng.randrange(16)) if rng.random() < 0.3 else v for v in (A, B))
+        t = dtype(rng.choice([BF16, F32]))
+        bias = bias if rng.random() < 0.5 else None
+        guarded = Guarded(rng, M, N, t)
+        ops.mm_int8_per_token(A, B, sa, sb, bias, out_dtype=t, out=guarded.out)
+        want, bound = mm_expected(A, B, sa, sb, bias, t)
+        assert_within(guarded.out, want, bound)
+        guarded.check()
+    assert ops.status() == 0
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_random_producers(ops, seed):
+    rng = random.Random(100 + seed)
+    for i in range(150):
+        C = spread(rng, 1, 30000)
+        N = spread(rng, 1, max(1, min(3000, 4000000 // C)))
+        if rng.random() < 0.5:
+            C = (C + 7) // 8 * 8
+        x_type = rng.choice([F16, BF16, F32])
+        g = generator(1000 * seed + i)
+        kind = rng.choice(["plain", "pairs", "halves", "norm"])
+        guarded = Guarded(rng, N, C, torch.int8)
+        if kind == "norm":
+            types = (x_type, rng.choice([x_type, F32]), rng.choice([x_type, F32]))
+            x, r, w, p, gt = norm_inputs(N, C, *types, rng.choice(["none", "channel", "scalar", "rows", "tokens"]), i)
+            p = p if rng.random() < 0.5 else None
+            x, r = (placed(v, rng.randrange(8)) if rng.random() < 0.3 else v for v in (x, r))
+            y64, dy, z64, dz = norm_expected(x, r, w, p, gt, 1e-5, 0.75)
+            y, z = ops.block_norm(x, r, w, 1e-5, post_weight=p, gate=gt, residual_scale=0.75)
+            assert_within(z, z64, dz + half_step(z64, z.dtype) * 1.01)
+            assert_within(y, y64, dy + half_step(y64, y.dtype) * 1.01)
+            q, s, z2 = ops.block_norm_quant_per_token(x, r, w, 1e-5, post_weight=p, gate=gt, residual_scale=0.75,
+                                                      out=guarded.out)
+            assert torch.equal(z, z2)
+            check_quantised(q, s, y64, dy)
+        else:
+            width, extra = (C if kind == "plain" else 2 * C), rng.choice([0, 0, 1, 5, 8])
+            wide = (torch.randn(N, width + extra, generator=g, device="cuda") * rng.choice([0.01, 3, 30])).to(dtype(x_type))
+            x = wide[:, :width] if rng.random() < 0.5 else wide[:, extra:]
+            if kind == "plain":
+                q, s = ops.quant_per_token(x, out=guarded.out)
+                check_quantised(q, s, x.double(), torch.zeros_like(x, dtype=torch.float64))
+            else:
+                q, s = ops.swiglu_quant_per_token(x, interleaved=kind == "pairs", out=guarded.out)
+                gate, up = (x[:, 0::2], x[:, 1::2]) if kind == "pairs" else (x[:, :C], x[:, C:])
+                gate, up = gate.double(), up.double()
+                y = gate / (1 + torch.exp(-gate)) * up
+                check_quantised(q, s, y, y.abs() * (1.24 * gate.abs().clamp_max(90) + 12) * U + 2.0 ** -114)
+        guarded.check()
